@@ -251,6 +251,75 @@ typedef struct m5_sample_params {
 M5_API int m5_sample_bf16(void* logits, int rows, int64_t vocab, int64_t ld, int32_t* history, int hist_len,
                           int64_t hist_ld, const m5_sample_params* p, uint64_t* state, int32_t* out, void* stream);
 
+/* ------------------------------------------------- speculative token trees
+ * Operators of speculative decoding over a tree of drafted tokens (no
+ * counterpart in the reference, whose speculation is a single chain).  A
+ * sequence b has lengths[b] committed keys in its cache rows [0, lengths[b]);
+ * node i of its tree (0 <= i < T <= 64, parents before children, node 0 the
+ * root) has its key and value in row lengths[b] + i. */
+
+/* ancestors[b][i] = bits of node i and of every node above it, depths[b][i] =
+ * nodes above it (depths may be NULL).  parents int32 [B, T]: -1 is a root; a
+ * node whose parent is neither -1 nor an earlier node (padding), or that hangs
+ * below such a node, gets 0 and depth 0. */
+M5_API int m5_tree_plan(const int32_t* parents, int B, int T, int64_t* ancestors, int32_t* depths, void* stream);
+
+/* Bytes of workspace m5_tree_attention needs for these shapes on the current
+ * device (any lengths, tree and bits). */
+M5_API int m5_tree_attention_workspace(int B, int Hq, int Hkv, int L, int D, size_t* bytes);
+
+/* out[b, h, i] = softmax(scale * q[b, h, i] @ K^T) @ V over the keys s <
+ * lengths[b] and the tree keys lengths[b] + j, j < tree_len, whose bit is set
+ * in ancestors[b][i]; 0 for a query that sees no key.  L <= 64 queries per
+ * sequence (all nodes, or the tree's newest ones; L = tree_len = 1 is the plain decoding
+ * step of sequences of different lengths), Hq a multiple of Hkv, D 64 or 128,
+ * bits 8/4 (groups of 64) or 0 (bf16).  q, out: bf16 with strides {batch,
+ * head, query} in elements (multiples of 8) and contiguous dims; keys, values:
+ * `capacity` rows per head, rows 16-byte aligned.  Keys at or above capacity
+ * do not exist.  Rows no query sees are not used, whatever they hold.  Scores,
+ * maxima and sums are fp32; nothing is rounded to bf16 before the output.
+ * workspace: 16-byte aligned, not shared by calls that may overlap. */
+M5_API int m5_tree_attention(const void* q, const int64_t* q_strides, int B, int Hq, int L, int D, m5_kv_view keys,
+                             m5_kv_view values, int Hkv, int64_t capacity, const int32_t* lengths, int tree_len,
+                             const int64_t* ancestors, int64_t ancestors_stride, float scale, int group_size,
+                             int bits, void* out, const int64_t* out_strides, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Logits processors for B sequences of T rows each (T = 1: plain decoding),
+ * row b * T + t of logits / out [B * T, vocab] (bf16 or fp32, row strides ld /
+ * out_ld; out may be logits).  In fp32, rounded once at the end:
+ *   c = counts[b][w] + times w occurs among tokens[b][j], bit j of ancestors[b][t]
+ *   c > 0: v = v < 0 ? v * repetition : v / repetition; v -= presence; v -= frequency * c
+ *   v += bias (bias_values[b][e] of the last e with bias_ids[b][e] == w)
+ *   v = -inf where bit w % 32 of mask[row][w / 32] is 0
+ * counts int32 [B, counts_ld], penalties fp32 [B, 3] = {repetition, presence,
+ * frequency}, tokens int32 / ancestors int64 [B, T], bias ids / values [B,
+ * n_bias] (ids outside the vocabulary are unused), mask int32 [B * T,
+ * mask_ld]; each may be NULL (0 entries).  choices int32 [B * T] (may be NULL):
+ * first index of the row's largest value, -1 where every entry is -inf or NaN.
+ * vocab <= 524288, n_bias <= 1024. */
+M5_API int m5_process_logits(const void* logits, int64_t ld, void* out, int64_t out_ld, int dtype, int B, int T,
+                             int64_t vocab, const int32_t* counts, int64_t counts_ld, const float* penalties,
+                             const int32_t* tokens, const int64_t* ancestors, const int32_t* bias_ids,
+                             const float* bias_values, int n_bias, const int32_t* mask, int64_t mask_ld,
+                             int32_t* choices, void* stream);
+
+/* Accept drafted tokens: starting at node 0, go to the first child whose token
+ * equals picks[cur] (the model's choice after node cur) while there is one.
+ * path int32 [B, T] = the nodes passed (-1 behind them), accepted[b] = how
+ * many (at least 1), next[b] = picks of the last one.  counts (may be NULL,
+ * int32 [B, counts_ld >= vocab]) gains 1 for the token of every accepted node. */
+M5_API int m5_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t* picks, int B, int T,
+                          int32_t* path, int32_t* accepted, int32_t* next, int32_t* counts, int64_t counts_ld,
+                          int64_t vocab, void* stream);
+
+/* Keep an accepted path in the caches: for every layer, head and i <
+ * accepted[b], row lengths[b] + path[b][i] of K and V (codes, scales, biases) is
+ * copied to row lengths[b] + i, in place.  layers: [B, Hkv, capacity, ...]
+ * buffers; rows at or above a layer's capacity are left alone. */
+M5_API int m5_tree_commit(const m5_layer_kv* layers, int num_layers, int B, int Hkv, int D, const int32_t* lengths,
+                          const int32_t* path, int T, const int32_t* accepted, void* stream);
+
 /* Qwen3-MoE router for T tokens: logits = x @ gate^T (w4g64), probabilities =
  * softmax (fp32 math, bf16 result), top-k by probability (ties -> lower
  * expert id), renormalised when norm_topk_prob.  ids int32 [T, k], scores

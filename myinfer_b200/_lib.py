@@ -84,6 +84,18 @@ _SIGS = {
     "m5_argmax_bf16": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "m5_sample_bf16": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_int64,
                                POINTER(M5SampleParams), c_void_p, c_void_p, c_void_p]),
+    "m5_tree_plan": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "m5_tree_attention_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, POINTER(c_size_t)]),
+    "m5_tree_attention": (c_int, [c_void_p, POINTER(c_int64), c_int, c_int, c_int, c_int, M5KvView, M5KvView, c_int,
+                                  c_int64, c_void_p, c_int, c_void_p, c_int64, c_float, c_int, c_int, c_void_p,
+                                  POINTER(c_int64), c_void_p, c_size_t, c_void_p]),
+    "m5_process_logits": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int64, c_void_p,
+                                  c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                  c_int64, c_void_p, c_void_p]),
+    "m5_tree_accept": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_int64, c_int64, c_void_p]),
+    "m5_tree_commit": (c_int, [POINTER(M5LayerKv), c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                               c_void_p]),
     "m5_moe_route": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                              c_void_p, c_void_p, c_void_p, c_void_p]),
     "m5_comm_unique_id": (c_int, [c_void_p, c_size_t]),

@@ -1,0 +1,503 @@
+"""The tree-speculation operators (myinfer_b200.tree) against their definitions in 64 bits.
+
+Attention's tolerance, per output element, from the roundings the kernel may
+make (u = 2^-11, fp16's unit roundoff): a key element that is used in fp16 is
+off by at most u times the largest value its conversion passes through (the
+value itself for 8-bit and bf16 caches, |bias| + 32 scale for 4-bit ones, whose
+conversion starts from 16 + code), and the D independent errors of a score add
+up like their root sum of squares; 8 / sqrt(3) of it is no less than 8 standard
+deviations.  A score off by d changes every weight by a factor in exp(+-2d).  Weights and values in
+fp16 add 2 u, fp32 sums less than u more.  The output's rounding to bf16 is half a unit, at most
+2^-8 of the value.  So
+  |d| <= 2^-8 |ref| + (2 d + 4 u) sum(p |v|) + u_v,  u_v = 2 u (|bias| + 32 scale) for 4-bit values,
+and in the 2-norm, over everything, 5e-3 (bf16 rounding alone is 1.7e-3)."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import tree as ref
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -11
+
+
+def _bf(x):
+    return torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).to(torch.bfloat16)
+
+
+def _f64(t):
+    return t.double().cpu().numpy()
+
+
+def _pack(x, bits):
+    """numpy fp32 [..., D] -> MLX tuple of torch CPU tensors."""
+    g = x.reshape(*x.shape[:-1], -1, 64)
+    lo, hi = g.min(-1), g.max(-1)
+    s, b = _bf((hi - lo) / (2 ** bits - 1)), _bf(lo)
+    sf, bfv = s.float().numpy(), b.float().numpy()
+    with np.errstate(divide="ignore", invalid="ignore"):
+        c = np.nan_to_num((g - bfv[..., None]) / sf[..., None])
+    c = np.clip(np.rint(c), 0, 2 ** bits - 1).astype(np.uint32).reshape(*x.shape[:-1], -1, 32 // bits)
+    w = np.zeros(c.shape[:-1], np.uint32)
+    for i in range(32 // bits):
+        w |= c[..., i] << np.uint32(bits * i)
+    return torch.from_numpy(w.view(np.int32)), s, b
+
+
+def _cache(rng, B, H, rows, D, bits, size=1.0):
+    x = (size * rng.standard_normal((B, H, rows, D))).astype(np.float32)
+    return _pack(x, bits) if bits else _bf(x)
+
+
+def _dense(t, bits):
+    """(fp64 values, fp64 bound of the magnitudes an fp16 conversion passes through) of a CPU cache."""
+    if not bits:
+        x = _f64(t)
+        return x, np.abs(x)
+    w, s, b = t[0].numpy(), _f64(t[1]), _f64(t[2])
+    x = ref.dequant((w, s, b), bits)
+    return x, np.abs(x) if bits == 8 else np.repeat(np.abs(b) + 32 * s, 64, -1)
+
+
+def _cuda(t):
+    return tuple(x.cuda() for x in t) if isinstance(t, tuple) else t.cuda()
+
+
+def _trees(rng, B, T):
+    p = np.full((B, T), -1, np.int32)
+    for i in range(1, T):
+        p[:, i] = rng.integers(max(0, i - 5), i, B)
+    return p
+
+
+def _attend(q, k, v, lengths, words, scale, T, bits, **kw):
+    from myinfer_b200.tree import tree_attention
+    return tree_attention(q, _cuda(k), _cuda(v), torch.tensor(lengths, dtype=torch.int32).cuda(),
+                          torch.from_numpy(words.view(np.int64).copy()).cuda(), scale, tree_len=T, bits=bits, **kw)
+
+
+def _check(out, q, k, v, lengths, words, scale, T, bits):
+    out, q = _f64(out), _f64(q)
+    (kd, km), (vd, vm) = _dense(k, bits), _dense(v, bits)
+    B, Hq, L, D = q.shape
+    Hk = kd.shape[1]
+    num = den = 0.0
+    for b in range(B):
+        end = min(lengths[b] + T, kd.shape[2])
+        kb, vb = (np.nan_to_num(x[b, :, :end], nan=0, posinf=0, neginf=0) for x in (kd, vd))
+        kmb, vmb = (np.nan_to_num(x[b, :, :end], nan=0, posinf=0, neginf=0) for x in (km, vm))
+        want, mag = ref.attention(q[b], kb, vb, lengths[b], words[b], T, scale)
+        tol = 2.0 ** -8 * np.abs(want) + 1e-30
+        for h in range(Hq):
+            hk = h // (Hq // Hk)
+            if end:
+                d = 8 / math.sqrt(3) * U * abs(scale) * np.sqrt((q[b, h] ** 2) @ (kmb[hk] ** 2).T).max(1)
+                tol[h] += (np.expm1(np.minimum(2 * d, 1.0)) + 4 * U)[:, None] * mag[h]
+                if bits == 4:
+                    tol[h] += 2 * U * vmb[hk].max(0)[None]
+        assert np.isfinite(out[b]).all()
+        err = np.abs(out[b] - want)
+        assert (err <= tol).all(), (b, float((err - tol).max()), np.argwhere(err > tol)[:4])
+        num, den = num + (err ** 2).sum(), den + (want ** 2).sum()
+    if den:
+        assert math.sqrt(num / den) <= 5e-3, math.sqrt(num / den)
+
+
+GRID = [  # B, Hq, Hkv, L, T, lengths, spare rows
+    (1, 8, 8, 1, 1, [0], 3),            # the first token of an empty cache
+    (1, 2, 1, 1, 1, [1], 0),            # a cache that ends with the tree
+    (1, 16, 8, 1, 1, [63], 9),
+    (1, 64, 8, 1, 1, [1500], 0),
+    (3, 4, 4, 1, 1, [0, 64, 129], 1),   # plain decoding of different lengths
+    (2, 10, 2, 7, 7, [1, 700], 5),      # a group of five heads
+    (1, 32, 2, 5, 5, [513], 2),         # a group of sixteen
+    (1, 8, 2, 17, 17, [100], 0),        # 68 rows per kv head
+    (4, 8, 4, 13, 13, [0, 3, 250, 1023], 7),
+    (1, 64, 8, 64, 64, [333], 1),       # 512 rows per kv head
+    (1, 16, 1, 64, 64, [2100], 30),     # 1024 rows on one kv head
+    (2, 4, 2, 16, 31, [65, 31], 4),     # the newest 16 of 31 nodes
+    (1, 6, 3, 1, 64, [200], 0),
+    (17, 2, 1, 3, 3, [11 * i for i in range(17)], 6),
+]
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", GRID, ids=lambda s: "b%d_h%dx%d_l%d_t%d_n%d" % (*s[:5], max(s[5])))
+def test_attention(shape, D, bits):
+    B, Hq, Hk, L, T, lengths, spare = shape
+    rng = np.random.default_rng(sum(lengths) + 7 * D + bits)
+    rows = max(lengths) + T + spare
+    q = _bf(1.5 * rng.standard_normal((B, Hq, L, D))).cuda()
+    k, v = _cache(rng, B, Hk, rows, D, bits), _cache(rng, B, Hk, rows, D, bits)
+    words = ref.ancestors(_trees(rng, B, T))[0][:, T - L:]
+    out = _attend(q, k, v, lengths, words, D ** -0.5, T, bits)
+    _check(out, q, k, v, lengths, words, D ** -0.5, T, bits)
+    again = _attend(q, k, v, lengths, words, D ** -0.5, T, bits)
+    assert torch.equal(out, again)  # no order of CTAs changes a result
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+def test_attention_masks_and_garbage(bits):
+    """Rows that see nothing are zero; rows nobody sees may hold NaN and infinities."""
+    rng = np.random.default_rng(5)
+    B, Hq, Hk, L, T, D = 2, 6, 2, 9, 9, 128
+    lengths, rows = [0, 130], 150
+    q = _bf(rng.standard_normal((B, Hq, L, D))).cuda()
+    k, v = _cache(rng, B, Hk, rows, D, bits), _cache(rng, B, Hk, rows, D, bits)
+    words = ref.ancestors(_trees(rng, B, T))[0]
+    dead = 4  # a node no one sees, and a query that sees nothing
+    words &= ~np.uint64(1 << dead)
+    words[:, 2] = 0
+    for t in (k, v):
+        for x in (t[1:] if bits else [t]):
+            for b in range(B):
+                x[b, :, lengths[b] + dead] = math.nan
+                x[b, :, lengths[b] + T:] = math.inf
+                x[b, 0, lengths[b] + T:] = math.nan
+    out = _attend(q, k, v, lengths, words, D ** -0.5, T, bits)
+    assert (out[0, :, 2] == 0).all() and (out[1, :, 2] != 0).any()
+    _check(out, q, k, v, lengths, words, D ** -0.5, T, bits)
+    high = words | np.uint64(0xFFFF) << np.uint64(T)  # bits beyond the tree are no keys
+    assert torch.equal(out, _attend(q, k, v, lengths, high, D ** -0.5, T, bits))
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("ksize,vsize,scale", [(3e4, 1.0, 3e-6), (1e-6, 1e-6, 8e4), (1.0, 3e5, 0.09), (1.0, 1.0, -0.09),
+                                               (40.0, 1.0, 0.09)])
+def test_attention_ranges(bits, ksize, vsize, scale):
+    """Keys and values far from 1, a negative scale, and scores of several hundred."""
+    rng = np.random.default_rng(11)
+    B, Hq, Hk, L, T, D = 1, 4, 2, 6, 6, 128
+    lengths = [391]
+    q = _bf(rng.standard_normal((B, Hq, L, D))).cuda()
+    k, v = _cache(rng, B, Hk, 400, D, bits, ksize), _cache(rng, B, Hk, 400, D, bits, vsize)
+    words = ref.ancestors(_trees(rng, B, T))[0]
+    _check(_attend(q, k, v, lengths, words, scale, T, bits), q, k, v, lengths, words, scale, T, bits)
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+def test_attention_growing_scores(bits):
+    """The running maximum moves at every tile, by more and less than the kernel may defer; values grow by 2^12 along the cache."""
+    rng = np.random.default_rng(12)
+    L = T = 3
+    n, D = 900, 64
+    grow = np.linspace(0.1, 9.0, n + T)[None, None, :, None]
+    q = _bf(np.abs(rng.standard_normal((1, 2, L, D)))).cuda()
+    kx = (np.abs(rng.standard_normal((1, 1, n + T, D))) * grow).astype(np.float32)
+    vx = (rng.standard_normal((1, 1, n + T, D)) * 2.0 ** (12 * grow / 9)).astype(np.float32)
+    k, v = ((_pack(kx, bits), _pack(vx, bits)) if bits else (_bf(kx), _bf(vx)))
+    words = ref.ancestors(_trees(rng, 1, T))[0]
+    _check(_attend(q, k, v, [n], words, 0.125, T, bits), q, k, v, [n], words, 0.125, T, bits)
+
+
+def test_attention_strides_and_views():
+    """Queries in token-major order, an output in the same order, a cache that is a slice of a larger one."""
+    from myinfer_b200.tree import tree_attention
+    rng = np.random.default_rng(3)
+    B, Hq, Hk, L, D, bits = 2, 8, 2, 5, 128, 8
+    rows, lengths = 90, [40, 77]
+    k, v = _cache(rng, B + 1, Hk + 1, rows + 7, D, bits), _cache(rng, B + 1, Hk + 1, rows + 7, D, bits)
+    cut = lambda t: tuple(x.cuda()[1:, 1:, 3:3 + rows] for x in t)  # noqa: E731
+    tok = _bf(rng.standard_normal((B, L, Hq, D))).cuda()
+    q = tok.transpose(1, 2)
+    words = ref.ancestors(_trees(rng, B, L))[0]
+    store = torch.full((B, L, Hq, D), math.nan, dtype=torch.bfloat16, device="cuda")
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    anc = torch.from_numpy(words.view(np.int64).copy()).cuda()
+    out = tree_attention(q, cut(k), cut(v), n, anc, D ** -0.5, bits=bits, out=store.transpose(1, 2))
+    assert out.data_ptr() == store.data_ptr()
+    kc, vc = (tuple(x[1:, 1:, 3:3 + rows] for x in t) for t in (k, v))
+    _check(out, q, kc, vc, lengths, words, D ** -0.5, L, bits)
+    odd = torch.empty(q.numel() + 1, dtype=torch.bfloat16, device="cuda")[1:].view(q.shape).copy_(q)  # 2-byte aligned
+    assert torch.equal(out, tree_attention(odd, cut(k), cut(v), n, anc, D ** -0.5, bits=bits))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = tree_attention(q, cut(k), cut(v), n, anc, D ** -0.5, bits=bits)
+    s.synchronize()
+    assert torch.equal(out, other)
+
+
+def test_attention_capacity_and_odd_heads():
+    """A tree that would pass the cache's end sees what is there; head starts at odd rows (scales 2-byte aligned)."""
+    rng = np.random.default_rng(8)
+    for D, bits in ((64, 8), (64, 4), (128, 4), (64, 0)):
+        B, Hq, Hk, L, rows = 1, 6, 3, 6, 141
+        q = _bf(rng.standard_normal((B, Hq, L, D))).cuda()
+        k, v = _cache(rng, B, Hk, rows, D, bits), _cache(rng, B, Hk, rows, D, bits)
+        words = ref.ancestors(_trees(rng, B, L))[0]
+        for n in (138, 141):
+            _check(_attend(q, k, v, [n], words, D ** -0.5, L, bits), q, k, v, [n], words, D ** -0.5, L, bits)
+
+
+def test_attention_far_offsets():
+    """A head that starts more than 2^31 bytes and 2^30 elements into the cache."""
+    from myinfer_b200.tree import tree_attention
+    rng = np.random.default_rng(9)
+    D, rows, n, L = 128, 9_000_000, 300, 4
+    q = _bf(rng.standard_normal((1, 4, L, D))).cuda()
+    small = [_cache(rng, 1, 2, n + L, D, 0) for _ in range(2)]
+    big = []
+    for t in small:
+        x = torch.empty(1, 2, rows, D, dtype=torch.bfloat16, device="cuda")
+        x[:, :, :n + L] = t.cuda()
+        big.append(x)
+    words = ref.ancestors(_trees(rng, 1, L))[0]
+    out = tree_attention(q, big[0], big[1], torch.tensor([n], dtype=torch.int32).cuda(),
+                         torch.from_numpy(words.view(np.int64).copy()).cuda(), D ** -0.5, bits=0)
+    _check(out, q, small[0], small[1], [n], words, D ** -0.5, L, 0)
+
+
+def test_attention_in_a_graph():
+    """Captured once, replayed with other lengths: nothing of the call lives on the host."""
+    from myinfer_b200.tree import tree_attention
+    rng = np.random.default_rng(10)
+    L, D, bits = 5, 128, 4
+    q = _bf(rng.standard_normal((2, 8, L, D))).cuda()
+    k, v = _cache(rng, 2, 2, 600, D, bits), _cache(rng, 2, 2, 600, D, bits)
+    kc, vc = _cuda(k), _cuda(v)
+    words = ref.ancestors(_trees(rng, 2, L))[0]
+    n = torch.tensor([10, 300], dtype=torch.int32).cuda()
+    anc = torch.from_numpy(words.view(np.int64).copy()).cuda()
+    tree_attention(q, kc, vc, n, anc, 0.09, bits=bits)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = tree_attention(q, kc, vc, n, anc, 0.09, bits=bits)
+    for lengths in ([10, 300], [595, 0], [64, 65]):
+        n.copy_(torch.tensor(lengths, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        _check(out, q, k, v, lengths, words, 0.09, L, bits)
+
+
+def test_plan():
+    from myinfer_b200.tree import tree_plan
+    rng = np.random.default_rng(1)
+    for B, T in ((1, 1), (3, 2), (5, 33), (2, 64)):
+        p = _trees(rng, B, T)
+        if T > 20:
+            p[0, 9] = -1            # a second root
+            p[1, 7] = 7             # no earlier node: 7 and what hangs below it are no nodes
+            p[1, 15] = 7
+            p[1, 16] = 15
+            p[1, 17:20] = (40, -5, 19)
+        anc, depth = tree_plan(torch.from_numpy(p).cuda())
+        bits, d = ref.ancestors(p)
+        assert (anc.cpu().numpy().view(np.uint64) == bits).all() and (depth.cpu().numpy() == d).all()
+    chain = np.arange(-1, 63, dtype=np.int32)[None]
+    anc, depth = tree_plan(torch.from_numpy(chain).cuda())
+    assert anc[0, 63].item() == -1 and depth[0, 63].item() == 63
+
+
+def _logits_inputs(rng, B, T, V, dtype, n_bias, mask):
+    R = B * T
+    x = (3 * rng.standard_normal((R, V))).astype(np.float32)
+    x = torch.from_numpy(x).to(dtype)
+    counts = (rng.random((B, V)) < 0.2) * rng.integers(1, 5, (B, V))
+    pen = np.stack([1 + rng.random(B), rng.random(B) - 0.3, rng.random(B)], 1).astype(np.float32)
+    words = ref.ancestors(_trees(rng, B, T))[0]
+    tok = rng.integers(0, V, (B, T)).astype(np.int32)
+    if T > 3:
+        tok[:, T - 1] = tok[:, 0]   # a token twice on a path
+        tok[0, 1] = -1              # and none at all
+    ids = rng.integers(0, V, (B, n_bias)).astype(np.int32)
+    if n_bias > 4:
+        ids[:, -1] = ids[:, 0]      # the last entry of a token counts
+        ids[:, 2] = -1
+        ids[:, 3] = V
+        ids[0, 4] = tok[0, 0]       # a bias on a path's token
+    val = (4 * rng.standard_normal((B, n_bias))).astype(np.float32)
+    m = None
+    if mask:
+        m = rng.integers(-2 ** 31, 2 ** 31 - 1, (R, (V + 31) // 32)).astype(np.int32)
+        m[0] = 0                    # nothing left
+        if R > 1:
+            m[1] = -1
+    return x, counts.astype(np.int32), pen, tok, words, ids, val, m
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,T,V,n_bias,mask", [(1, 1, 1, 0, False), (1, 1, 1000, 0, True), (2, 5, 4099, 40, True),
+                                               (3, 1, 8191, 7, False), (1, 64, 4096, 300, True),
+                                               (2, 3, 40000, 1024, True), (1, 2, 151936, 5, True)])
+def test_process_logits(dtype, B, T, V, n_bias, mask):
+    """Every operation is one correctly rounded fp32 operation: at most 6 of them,
+    2^-24 each of the largest value on the way, then the logits' own rounding: the result lies
+    between the roundings of the exact value less and plus that error.  Choices are the first
+    largest of the values returned."""
+    from myinfer_b200.tree import process_logits
+    rng = np.random.default_rng(V + T)
+    x, counts, pen, tok, words, ids, val, m = _logits_inputs(rng, B, T, V, dtype, n_bias, mask)
+    up = lambda a: None if a is None else torch.from_numpy(a).cuda()  # noqa: E731
+    kw = dict(batch=B, counts=up(counts), penalties=up(pen), tokens=up(tok), ancestors=up(words.view(np.int64).copy()),
+              mask=up(m))
+    if n_bias:
+        kw.update(bias_ids=up(ids), bias_values=up(val))
+    lg = x.cuda()
+    out, choice = process_logits(lg, **kw)
+    assert out.dtype == dtype and torch.equal(lg.cpu(), x)
+    got, pick = _f64(out), choice.cpu().numpy()
+    rounded = lambda z: _f64(torch.from_numpy(z).to(dtype))  # noqa: E731
+    for r in range(B * T):
+        b, t = divmod(r, T)
+        path = [tok[b, j] for j in range(T) if int(words[b, t]) >> j & 1]
+        want = ref.process_row(_f64(x[r]), counts[b], pen[b], path, list(zip(ids[b], val[b])),
+                               None if m is None else m[r].view(np.uint32))
+        gone = np.isneginf(want)
+        assert (np.isneginf(got[r]) == gone).all()
+        big = 2 * np.abs(_f64(x[r])) + 1 + counts[b].astype(np.float64) + T + (np.abs(val[b]).max() if n_bias else 0)
+        e, y = 6 * 2.0 ** -24 * big[~gone], got[r][~gone]
+        assert (rounded(want[~gone] - e) <= y).all() and (y <= rounded(want[~gone] + e)).all(), r
+        assert pick[r] == ref.choice(got[r]), r
+    inplace, c2 = process_logits(lg, out=lg, **kw)
+    assert inplace is lg and torch.equal(lg, out) and torch.equal(c2, choice)
+
+
+def test_process_logits_strides_nan_and_ties():
+    from myinfer_b200.tree import process_logits
+    V = 5003
+    store = torch.full((3, V + 13), 7.0, dtype=torch.bfloat16, device="cuda")
+    lg = store[:, 5:5 + V]
+    lg.copy_(torch.zeros(3, V))
+    lg[0, 100], lg[0, 4000] = 2.0, 2.0             # a tie: the lowest index
+    lg[0, 50] = math.nan                           # never chosen
+    lg[1, 3] = -0.0
+    lg[1, :3] = -1.0                               # -0 ties with 0
+    lg[2] = math.nan
+    lg[2, 4999] = -3.0
+    out, c = process_logits(lg, out=lg)
+    assert c.tolist() == [100, 3, 4999] and out.data_ptr() == lg.data_ptr()
+    assert (store[:, :5] == 7).all() and (store[:, 5 + V:] == 7).all()
+    m = torch.full((3, (V + 31) // 32), -1, dtype=torch.int32, device="cuda")
+    m[0, 50 // 32] = 0                             # NaN and infinity in masked places
+    m[2] = 0
+    lg[2, 7] = math.inf
+    out, c = process_logits(lg, mask=m)
+    assert c.tolist() == [100, 3, -1] and not torch.isnan(out[0]).any() and torch.isneginf(out[2]).all()
+    lg[1, 17] = math.inf
+    assert process_logits(lg)[1][1].item() == 17
+    one, c = process_logits(lg[:1])                # one row of a wider tensor
+    assert c.item() == 100 and one.shape == (1, V)
+
+
+def test_process_logits_matches_greedy_sampler_without_processors():
+    from myinfer_b200 import ops
+    from myinfer_b200.tree import process_logits
+    x = torch.randn(1, 151936, device="cuda").to(torch.bfloat16)
+    out, c = process_logits(x)
+    assert torch.equal(out, x) and c.item() == ops.argmax(x[0]).item()
+
+
+@pytest.mark.parametrize("B,T", [(1, 1), (2, 2), (9, 17), (64, 64)])
+def test_accept(B, T):
+    from myinfer_b200.tree import tree_accept
+    rng = np.random.default_rng(T)
+    V = 50
+    p = _trees(rng, B, T)
+    tok = rng.integers(0, 6, (B, T)).astype(np.int32)   # few tokens: siblings with the same one
+    pick = rng.integers(0, 6, (B, T)).astype(np.int32)
+    if T > 5:
+        p[0, T - 2:] = -2                                # padding
+        pick[1, 0] = 49                                  # nothing accepted
+        p[-1], tok[-1], pick[-1] = np.arange(-1, T - 1), 3, 3  # a chain accepted to its end
+    counts = rng.integers(0, 9, (B, V)).astype(np.int32)
+    dev = [torch.from_numpy(a.copy()).cuda() for a in (p, tok, pick, counts)]
+    path, n, nxt = tree_accept(*dev[:3], counts=dev[3])
+    for b in range(B):
+        want, follow = ref.accept(p[b], tok[b], pick[b])
+        assert n[b].item() == len(want) and nxt[b].item() == follow
+        assert path[b].tolist() == want + [-1] * (T - len(want))
+        for i in want:
+            counts[b, tok[b, i]] += 1
+    assert (dev[3].cpu().numpy() == counts).all()
+    assert torch.equal(tree_accept(*dev[:3])[0], path)
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("D", [64, 128])
+def test_commit(bits, D):
+    from myinfer_b200.tree import CacheLayers, commit_tree
+    rng = np.random.default_rng(bits + D)
+    B, Hk, rows, T = 3, 2, 133, 64
+    path = np.full((B, T), -1, np.int32)
+    lens = np.array([0, 69, 75], np.int32)               # the last one's tree passes the end of the cache
+    for b, p in enumerate(([0, 1, 4, 5, 9, 63], list(range(64)), [0, 2, 40, 57, 58, 60])):
+        path[b, :len(p)] = p
+    n = np.array([6, 64, 6], np.int32)
+    layers, before = [], []
+    for _ in range(130):                                 # more layers than one launch takes
+        pair = []
+        for _ in range(2):
+            if bits:
+                pair.append((torch.randint(-2 ** 31, 2 ** 31 - 1, (B, Hk, rows, D * bits // 32), dtype=torch.int32,
+                                           device="cuda"),
+                             *[torch.randn(B, Hk, rows, D // 64, device="cuda").to(torch.bfloat16) for _ in range(2)]))
+            else:
+                pair.append(torch.randn(B, Hk, rows, D, device="cuda").to(torch.bfloat16))
+        layers.append(tuple(pair))
+        before.append([x.clone() for t in pair for x in (t if bits else (t,))])
+    table = CacheLayers(layers)
+    args = [torch.from_numpy(a).cuda() for a in (lens, path, n)]
+    commit_tree(table, *args)
+    for (k, v), old in zip(layers, before):
+        for x, o in zip((*k, *v) if bits else (k, v), old):
+            want = o.clone()
+            for b in range(B):
+                for i in range(n[b]):
+                    if lens[b] + max(path[b, i], i) < rows:
+                        want[b, :, lens[b] + i] = o[b, :, lens[b] + path[b, i]]
+            assert torch.equal(x, want)
+
+
+def test_refusals():
+    from myinfer_b200 import tree
+    dev = "cuda"
+    q = torch.zeros(1, 4, 2, 128, dtype=torch.bfloat16, device=dev)
+    k = torch.zeros(1, 2, 8, 128, dtype=torch.bfloat16, device=dev)
+    n = torch.zeros(1, dtype=torch.int32, device=dev)
+    a = torch.zeros(1, 2, dtype=torch.int64, device=dev)
+    ok = lambda **kw: tree.tree_attention(**{**dict(queries=q, q_keys=k, q_values=k, lengths=n, ancestors=a, scale=1.0,  # noqa: E731
+                                                    bits=0), **kw})
+    assert ok().shape == q.shape
+    wide = torch.zeros(1, 2, 8, 256, dtype=torch.bfloat16, device=dev)[..., :128]
+    shifted = torch.zeros(1 * 2 * 8 * 128 + 4, dtype=torch.bfloat16, device=dev)[4:].view(1, 2, 8, 128)
+    for kw in (dict(queries=q.float()), dict(queries=q.cpu()), dict(queries=q[..., :96]), dict(q_keys=wide),
+               dict(queries=torch.zeros(1, 4, 65, 128, dtype=torch.bfloat16, device=dev)), dict(tree_len=65),
+               dict(tree_len=0), dict(q_keys=k[:, :1]), dict(queries=q[:, :3]), dict(lengths=n.long()),
+               dict(lengths=torch.zeros(2, dtype=torch.int32, device=dev)), dict(ancestors=a.int()), dict(bits=8),
+               dict(bits=3), dict(q_values=k.half()), dict(lengths=n.cpu()), dict(out=torch.empty_like(q).float())):
+        with pytest.raises(ValueError):
+            ok(**kw)
+    from myinfer_b200._lib import M5CudaError
+    with pytest.raises(M5CudaError, match="aligned"):
+        ok(q_keys=shifted)
+    lg = torch.zeros(6, 100, dtype=torch.bfloat16, device=dev)
+    for kw in (dict(batch=4), dict(counts=torch.zeros(6, 100, dtype=torch.int32, device=dev)),
+               dict(bias_ids=torch.zeros(6, 1, dtype=torch.int32, device=dev)),
+               dict(mask=torch.zeros(6, 3, dtype=torch.int64, device=dev)), dict(out=lg.float()),
+               dict(tokens=torch.zeros(6, 1, dtype=torch.int32, device=dev))):
+        with pytest.raises(ValueError):
+            tree.process_logits(lg, **kw)
+    for bad in (lg.half(), lg.cpu(), lg.t(), lg[0]):
+        with pytest.raises(ValueError):
+            tree.process_logits(bad)
+    with pytest.raises(M5CudaError, match="mask"):
+        tree.process_logits(lg, mask=torch.zeros(6, 3, dtype=torch.int32, device=dev))
+    p = torch.zeros(2, 5, dtype=torch.int32, device=dev)
+    for bad in (p.cpu(), p.long(), p[0], torch.zeros(1, 65, dtype=torch.int32, device=dev)):
+        with pytest.raises(ValueError):
+            tree.tree_plan(bad)
+    with pytest.raises(ValueError):
+        tree.tree_accept(p, p[:, :4].contiguous(), p)
+    with pytest.raises(ValueError):
+        tree.tree_accept(p, p, p, counts=torch.zeros(3, 9, dtype=torch.int32, device=dev))
+    for bad in ([], [(wide, wide)], [(k, k[:, :, :4])], [(k.half(), k.half())], [(k, k), (k[:, :1].contiguous(),) * 2]):
+        with pytest.raises(ValueError):
+            tree.CacheLayers(bad)
+    with pytest.raises(ValueError):
+        tree.commit_tree([(k, k)], n, p, n)
