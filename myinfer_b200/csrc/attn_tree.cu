@@ -12,15 +12,15 @@
 // inside a (sequence, head, row block) leaves a partial (max, sum, O) in the
 // workspace, joined by tree_join_kernel.
 //
-// Roles of a CTA (480 threads):
-//   warp 13      producer: bulk copies of 64-key tiles of K / V rows and of their
+// Roles of a CTA (640 threads, registers moved to the softmax by setmaxnreg):
+//   warp 17      producer: bulk copies of 64-key tiles of K / V rows and of their
 //                scales and biases (as the 16-byte blocks around them, so any
 //                2-byte alignment will do) into a ring;
-//   warp 14      scales: per tile and operand the exponent that puts the tile's largest value
-//                into [2^7, 2^8), and scale and bias in fp16 under it;
-//   warps 8-11   conversion to fp16, K and V alike: [key][dim] rows of 128 bytes,
-//                128-byte swizzle (K is read K-major, V MN-major: no transpose);
-//   warp 12      one thread issues the MMAs:  S = Q K^T  (Q, K in shared memory) and
+//   warps 18-19  scales, even and odd tiles: per tile and operand the exponent that puts the tile's largest value
+//                under 2^-2, and scale and bias in fp16 under it;
+//   warps 8-15   conversion to fp16, four warps for K and four for V, both into [key][dim] rows of
+//                128 bytes, 128-byte swizzle (K is read K-major, V MN-major: no transpose);
+//   warp 16      one thread issues the MMAs:  S = Q K^T  (Q, K in shared memory) and
 //                O += P V  (P in tensor memory);
 //   warps 0-7    softmax.  Even and odd tiles are two independent streams of four
 //                warps each, with their own running maximum, sum and O, so that one's exponentials
@@ -28,8 +28,8 @@
 //                stream and P overwrites the S it came from.
 // Rounding: K, V and P are fp16 (2^-12 of the value or less; bf16 would cost as
 // much as the output's own rounding).  The exponents make that safe for
-// any range: values keep full precision down to 2^-22 of their tile's largest
-// one.  Q is scaled per row in the same way, which is exact.  Scores, maxima,
+// any range: an element's absolute error is at most 2^-23 of its tile's largest
+// value.  Q is scaled per row in the same way, which is exact.  Scores, maxima,
 // sums and O are fp32.  A row's maximum is only moved when a new score exceeds
 // it by 2^8 (p <= 256 in fp16): O is rescaled rarely.
 // With 64 rows or fewer, the idle rows repeat the rows and take a part of each
@@ -50,15 +50,22 @@ namespace atr {
 
 constexpr int TK = 64;      // keys per tile
 constexpr int ROWS = 128;   // MMA M
-constexpr int SMX_WARPS = 8, DQ_WARPS = 4;
-constexpr int MMA_WARP = SMX_WARPS + DQ_WARPS, PROD_WARP = MMA_WARP + 1, PREP_WARP = MMA_WARP + 2;
-constexpr int THREADS = (PREP_WARP + 1) * 32;
+constexpr int SMX_WARPS = 8, DQ_WARPS = 4;  // conversion: DQ_WARPS for K and as many for V
+constexpr int MMA_WARP = SMX_WARPS + 2 * DQ_WARPS, PROD_WARP = MMA_WARP + 1, PREP_WARP = MMA_WARP + 2;
+constexpr int THREADS = (PREP_WARP + 2) * 32;
+// registers per thread after setmaxnreg: 2 + 2 + 1 warpgroups out of 640 x 96 at launch
+constexpr int SMX_REGS = 136, DQ_REGS = 72, MISC_REGS = 56;
+static_assert(256 * SMX_REGS + 256 * DQ_REGS + 128 * MISC_REGS <= 640 * 96, "register split");
 constexpr int NOP = 3;      // converted K and V tiles held
 constexpr int EXPS = 32;    // tile exponents held: more than the tiles between conversion and softmax
 constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LAZY = 8.f; // log2 growth of a row's maximum that is left in p
-constexpr int TOP = 7;      // exponent of a tile's largest value in fp16
+// Exponent of the largest value in fp16: of a bf16 row or tile, and of a packed
+// tile.  Codes are used as fp16 subnormals (code * 2^-24, 4-bit: * 2^-20), an
+// exact operand without a conversion; scale * 2^24 stays finite when the tile's values,
+// hence 255 scales, stay below 2^-1.
+constexpr int TOP16 = 7, TOPQ = -3;
 constexpr int MIN_TILES = 2;  // per CTA: one per stream
 
 template <int BITS, int D>
@@ -86,7 +93,7 @@ struct Bars {
   uint64_t sfull[4];   // [stream][buffer]
   uint64_t pfull[2], pvdone[2];
   uint64_t qready, idle;
-  uint64_t dqmax;      // bf16 caches: the conversion warps' maxima of a tile are in shared memory
+  uint64_t dqmax[2];   // [K, V] bf16 caches: the conversion warps' maxima of a tile are in shared memory
 };
 
 __device__ __forceinline__ uint32_t sw128(int n, int j) {
@@ -95,11 +102,6 @@ __device__ __forceinline__ uint32_t sw128(int n, int j) {
 __device__ __forceinline__ uint32_t h2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t hsub1024(uint32_t x) {
-  uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64006400u));
   return r;
 }
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
@@ -118,10 +120,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }  // |e| <= 126
-// e with max / 2^e in [2^TOP, 2^(TOP + 1)), kept to exponents pow2 can hold
-__device__ __forceinline__ int top_exp(float max) {
-  const int e = int(__float_as_uint(max) >> 23) - 127 - TOP;
-  return ::min(120, ::max(-120, e));
+// e with max / 2^e in [2^top, 2^(top + 1)), kept to exponents whose powers are finite
+__device__ __forceinline__ int top_exp(float max, int top) {
+  const int e = int(__float_as_uint(max) >> 23) - 127 - top;
+  return ::min(120, ::max(-100, e));
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -135,65 +137,74 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lead) {
   return tc_sdesc_sw128(addr) & ~(uint64_t(0x3FFF) << 16) | (uint64_t(lead >> 4) << 16);
 }
 
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
 }
-// Bounded wait by one thread (~2 s); a failure is shared by the CTA.
+// Bounded wait by one thread (M5_WAIT_LIMIT polls of up to ~2 us); a failure is shared by the CTA.
 __device__ __forceinline__ bool wait1(uint64_t* bar, uint32_t par, volatile int* fail) {
-  if (mbar_try_wait_fast(bar, par)) return true;
-  const uint64_t t0 = now_ns();
-  for (;;) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < M5_WAIT_LIMIT; ++i) {
     if (mbar_try_wait(bar, par)) return true;
     if (*fail) return false;
-    if (now_ns() - t0 > 2000000000ull) break;
   }
   *fail = 1;
   atomicExch(&g_attn_tree_err, M5_DEV_ERR_WAIT_TIMEOUT);
   return false;
 }
-// Bounded wait by a warp: every lane polls, the result is the same for all.
+// by a warp: every lane polls, the result is the same for all
 __device__ __forceinline__ bool waitw(uint64_t* bar, uint32_t par, volatile int* fail) {
   return __all_sync(0xffffffffu, wait1(bar, par, fail));
 }
 
+// A slot of a ring of N buffers and the parity of its current use.
+template <int N>
+struct Slot {
+  int i = 0;
+  uint32_t par = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
+      par ^= 1;
+    }
+  }
+};
+
 // The line of tiles: sequences in order, each with `pairs` (kv head, row
-// block) runs of tiles(b) tiles.
+// block) runs of tiles(b) tiles.  32-bit counts: the host refuses longer lines.
 struct Line {
-  long long total, begin, end;  // all tiles; this CTA's part
-  int b;                        // sequence of `begin` and where its tiles start
-  long long base;
+  int begin, end;  // this CTA's part
+  int b, base;     // sequence of tile `begin`, and that sequence's first tile
 };
 __device__ __forceinline__ int seq_len(const TreeAttnArgs& a, int b) {
-  return (int)::min((long long)::max(a.lengths[b], 0), (long long)a.capacity);
+  return ::min(::max(a.lengths[b], 0), (int)a.capacity);
 }
-__device__ __forceinline__ int seq_end(const TreeAttnArgs& a, int n) {
-  return (int)::min((long long)n + a.T, (long long)a.capacity);
-}
+__device__ __forceinline__ int seq_end(const TreeAttnArgs& a, int n) { return ::min(n + a.T, (int)a.capacity); }
 __device__ __forceinline__ int seq_tiles(const TreeAttnArgs& a, int b) {
   return (seq_end(a, seq_len(a, b)) + TK - 1) / TK;
 }
-__device__ __forceinline__ long long part_of(long long total, int ctas, long long c) { return total * c / ctas; }
-__device__ __forceinline__ int parts(const TreeAttnArgs& a, long long total, int ctas) {
-  return (int)::min((long long)ctas, ::max(1LL, total / MIN_TILES));
-}
-// by one warp: the sum over all sequences, and the sequence that holds tile `at`
-// (at < 0: none wanted)
-__device__ __forceinline__ void scan_line(const TreeAttnArgs& a, int pairs, int lane, long long at, long long& total,
-                                          int& b_at, long long& base_at) {
-  long long sum = 0;
+__device__ __forceinline__ int part_of(int total, int ctas, int c) { return (int)((long long)total * c / ctas); }
+__device__ __forceinline__ int parts(int total, int ctas) { return ::min(ctas, ::max(1, total / MIN_TILES)); }
+// by one warp: the tiles of all sequences; b_at and base_at: the sequence that
+// holds tile `at`, if any does
+__device__ __forceinline__ int scan_line(const TreeAttnArgs& a, int pairs, int lane, int at, int& b_at, int& base_at) {
+  int sum = 0;
+#pragma unroll 1
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int b = b0 + lane;
-    const long long w = b < a.B ? (long long)seq_tiles(a, b) * pairs : 0;
-    long long inc = w;
+    const int w = b < a.B ? seq_tiles(a, b) * pairs : 0;
+    int inc = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+      const int u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
-    const bool here = at >= sum + inc - w && at < sum + inc;
-    const unsigned m = __ballot_sync(0xffffffffu, here);
+    const unsigned m = __ballot_sync(0xffffffffu, at >= sum + inc - w && at < sum + inc);
     if (m) {
       const int src = __ffs(m) - 1;
       b_at = b0 + src;
@@ -201,42 +212,39 @@ __device__ __forceinline__ void scan_line(const TreeAttnArgs& a, int pairs, int 
     }
     sum += __shfl_sync(0xffffffffu, inc, 31);
   }
-  total = sum;
+  return sum;
 }
 
 // Walks a CTA's part run by run; every role holds one and steps it alike.
 struct Walk {
-  long long at, end, base;
-  int b, n, kend, tiles;                      // sequence: committed keys, end of its keys, tiles
-  int hk, rb, t0, nt, pair;                   // run: kv head, row block, first tile, tiles of this part; pair = its number
-  bool whole;                                 // the part holds all of the run
-  __device__ __forceinline__ Walk(const Line& l, const TreeAttnArgs& a) : at(l.begin), end(l.end), base(l.base), b(l.b) {
-    load(a);
-  }
-  __device__ __forceinline__ void load(const TreeAttnArgs& a) {
-    n = seq_len(a, b);
-    kend = seq_end(a, n);
-    tiles = (kend + TK - 1) / TK;
-  }
+  int at, end, base;
+  int b, n, kend, tiles;        // sequence: committed keys, end of its keys, tiles
+  int hk, rb, t0, nt, pair;     // run: kv head, row block, first tile, tiles of this part; pair = its number
+  __device__ __forceinline__ Walk(const Line& l, const TreeAttnArgs& a)
+      : at(l.begin), end(l.end), base(l.base), b(l.b), tiles(0) {}
   __device__ __forceinline__ bool next(const TreeAttnArgs& a, int nrb) {
     if (at >= end) return false;
     const int pairs = a.Hkv * nrb;
-    if (at - base >= (long long)tiles * pairs) {
-      base += (long long)tiles * pairs;
+    if (tiles && at - base >= tiles * pairs) {
+      base += tiles * pairs;
       ++b;
-      load(a);
+      tiles = 0;
     }
-    const long long in = at - base;
-    const int p = (int)(in / tiles);
-    t0 = (int)(in - (long long)p * tiles);
-    nt = (int)::min((long long)(tiles - t0), end - at);
-    hk = p / nrb;
-    rb = p % nrb;
+    if (!tiles) {
+      n = seq_len(a, b);
+      kend = seq_end(a, n);
+      tiles = (kend + TK - 1) / TK;
+    }
+    const unsigned in = at - base, p = in / (unsigned)tiles;
+    t0 = in - p * tiles;
+    nt = ::min(tiles - t0, end - at);
+    hk = nrb == 1 ? p : p / (unsigned)nrb;
+    rb = p - hk * nrb;
     pair = b * pairs + p;
-    whole = t0 == 0 && nt == tiles;
     at += nt;
     return true;
   }
+  __device__ __forceinline__ bool whole() const { return nt == tiles; }
 };
 
 // Rows of a block (nrows of 128) repeat 4, 2 or 1 times over the lanes.
@@ -261,26 +269,18 @@ __device__ __forceinline__ unsigned long long visible(unsigned long long word, i
 }
 
 // fp16 (K, V): 8 consecutive dims of a row into one 16-byte chunk.
-// 8-bit: (1024 + code) - 1024 is exact, as are s and b (bf16 values), so code * s + b is rounded
-// once.  Folding an offset of the code into b instead would round b, which errs alike for
-// all 64 dims of a group: 1 % of the output where the scores reach 50.
+// 8-bit: byte c is the fp16 subnormal c * 2^-24; s (times 2^24) and b are exact
+// (bf16 values), so code * s + b is rounded once.  An offset of the code folded into b
+// instead would round b, which errs alike for all 64 dims of a group: 1 % of the
+// output where the scores reach 50.
 __device__ __forceinline__ uint4 conv8(uint2 w, uint32_t s, uint32_t b) {
-  uint4 o;
-  o.x = hfma2(hsub1024(__byte_perm(w.x, 0x64u, 0x4140)), s, b);
-  o.y = hfma2(hsub1024(__byte_perm(w.x, 0x64u, 0x4342)), s, b);
-  o.z = hfma2(hsub1024(__byte_perm(w.y, 0x64u, 0x4140)), s, b);
-  o.w = hfma2(hsub1024(__byte_perm(w.y, 0x64u, 0x4342)), s, b);
-  return o;
+  return make_uint4(hfma2(__byte_perm(w.x, 0u, 0x4140), s, b), hfma2(__byte_perm(w.x, 0u, 0x4342), s, b),
+                    hfma2(__byte_perm(w.y, 0u, 0x4140), s, b), hfma2(__byte_perm(w.y, 0u, 0x4342), s, b));
 }
-// 4-bit: the same.  Position 2 i + h of the chunk is dim i + 4 h.
+// 4-bit: nibble c at bits 4-7 is c * 2^-20.  Position 2 i + h of the chunk is dim i + 4 h.
 __device__ __forceinline__ uint4 conv4(uint32_t w, uint32_t s, uint32_t b) {
-  constexpr uint32_t M = 0x000F000Fu, X = 0x64006400u;
-  uint4 o;
-  o.x = hfma2(hsub1024((w & M) | X), s, b);
-  o.y = hfma2(hsub1024(((w >> 4) & M) | X), s, b);
-  o.z = hfma2(hsub1024(((w >> 8) & M) | X), s, b);
-  o.w = hfma2(hsub1024(((w >> 12) & M) | X), s, b);
-  return o;
+  constexpr uint32_t M = 0x00F000F0u;
+  return make_uint4(hfma2((w << 4) & M, s, b), hfma2(w & M, s, b), hfma2((w >> 4) & M, s, b), hfma2((w >> 8) & M, s, b));
 }
 __device__ __forceinline__ uint4 conv16(uint4 w, float f) {
   return make_uint4(h2(bf16_lo(w.x) * f, bf16_hi(w.x) * f), h2(bf16_lo(w.y) * f, bf16_hi(w.y) * f),
@@ -304,21 +304,38 @@ struct Row {
   int ev;      // O holds its sum divided by 2^ev
 };
 
-// One tile of a softmax thread: N of the tile's 64 keys, from `off` on.  P of the
-// other keys is zero.  Returns false when a wait failed.
-template <int N, int D>
-__device__ __forceinline__ bool softmax_tile(Row& r, uint32_t s_addr, uint32_t o_addr, int off, float c, int ev,
-                                             bool edge, unsigned long long vis, bool first, uint64_t* pvdone,
-                                             uint32_t pv_par, volatile int* fail) {
-  float s[N];
+// O *= f for this thread's row.
+template <int D>
+__device__ __forceinline__ void scale_o(uint32_t o_addr, float f) {
+#pragma unroll 1
+  for (int d = 0; d < D; d += 32) {
+    float o[32];
+    tmem_ld32(o_addr + d, o);
+    tmem_ld_wait();
 #pragma unroll
-  for (int i = 0; i < N; i += 16) tmem_ld16(s_addr + off + i, *reinterpret_cast<float(*)[16]>(s + i));
+    for (int i = 0; i < 32; ++i) o[i] *= f;
+    tmem_st32(o_addr + d, reinterpret_cast<const uint32_t*>(o));
+  }
+}
+
+// One tile of a softmax thread: N of the tile's 64 keys, from `off` on; P of the
+// other keys is zero.  Returns the factor by which O has to change.
+template <int N>
+__device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, float c, bool edge,
+                                              unsigned long long vis) {
+  float s[N];
+  if constexpr (N == 16) {
+    tmem_ld16(s_addr + off, s);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 32) tmem_ld32(s_addr + off + i, *reinterpret_cast<float(*)[32]>(s + i));
+  }
   tmem_ld_wait();
   if (edge) {
-    vis >>= off;
+    const uint32_t v[2] = {uint32_t(vis >> off), uint32_t((vis >> off) >> 32)};
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (!((vis >> i) & 1)) s[i] = -INFINITY;
+      if (!((v[i / 32] >> (i % 32)) & 1)) s[i] = -INFINITY;
   }
   float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -329,13 +346,11 @@ __device__ __forceinline__ bool softmax_tile(Row& r, uint32_t s_addr, uint32_t o
   const float tmax = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
   const float mt = tmax == -INFINITY ? -INFINITY : tmax * c;
   float corr = 1.f;
-  if (mt > r.m + LAZY || (r.m == -INFINITY && mt != -INFINITY)) {
+  if (mt > r.m + LAZY) {  // also: the first score the row sees (r.m = -inf)
     corr = r.m == -INFINITY ? 0.f : ex2(r.m - mt);
     r.m = mt;
     r.l *= corr;
   }
-  if (!first && ev != r.ev) corr *= pow2(::max(r.ev - ev, -126));
-  r.ev = ev;
   const float neg = r.m == -INFINITY ? 0.f : -r.m;
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   uint32_t p[N / 2];
@@ -361,22 +376,7 @@ __device__ __forceinline__ bool softmax_tile(Row& r, uint32_t s_addr, uint32_t o
       tmem_st16(s_addr + k / 2, z);
     }
   }
-  if (!first && __any_sync(0xffffffffu, corr != 1.f)) {
-    if (!waitw(pvdone, pv_par, fail)) return false;
-    tc_fence_after();
-#pragma unroll
-    for (int d = 0; d < D; d += 16) {
-      float o[16];
-      uint32_t u[16];
-      tmem_ld16(o_addr + d, o);
-      tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * corr);
-      tmem_st16(o_addr + d, u);
-    }
-  }
-  tmem_st_wait();
-  return true;
+  return corr;
 }
 
 template <int BITS, int D>
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     s_fail = 0;
     for (int i = 0; i < ST; ++i) {
       mbar_init(&bar.full[i], 1);
-      mbar_init(&bar.empty[i], DQ_WARPS);
+      mbar_init(&bar.empty[i], 2 * DQ_WARPS);
       mbar_init(&bar.prep[i], 1);
     }
     for (int i = 0; i < NOP; ++i) {
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     }
     mbar_init(&bar.qready, SMX_WARPS);
     mbar_init(&bar.idle, 1);
-    mbar_init(&bar.dqmax, DQ_WARPS);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.dqmax[i], DQ_WARPS);
     fence_mbar_init();
   }
   if (warp == MMA_WARP) {
@@ -432,15 +432,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     tmem_relinquish();
   }
   if (warp == 0) {
-    Line l;
-    scan_line(a, a.Hkv * nrb, lane, -1, l.total, l.b, l.base);
-    const int np = parts(a, l.total, gridDim.x), c = blockIdx.x;
-    l.begin = c < np ? part_of(l.total, np, c) : l.total;
-    l.end = c < np ? part_of(l.total, np, c + 1) : l.total;
-    l.b = a.B - 1;
-    l.base = 0;
-    long long t;
-    scan_line(a, a.Hkv * nrb, lane, l.begin, t, l.b, l.base);
+    Line l{0, 0, a.B - 1, 0};
+    const int total = scan_line(a, a.Hkv * nrb, lane, -1, l.b, l.base);
+    const int np = parts(total, gridDim.x), c = blockIdx.x;
+    l.begin = c < np ? part_of(total, np, c) : total;
+    l.end = c < np ? part_of(total, np, c + 1) : total;
+    scan_line(a, a.Hkv * nrb, lane, l.begin, l.b, l.base);
     if (lane == 0) s_line = l;
   }
   tc_fence_before();
@@ -450,68 +447,80 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
   const Line line = s_line;
   const int cta_slot = blockIdx.x;
 
+  if (warp >= MMA_WARP) setmaxnreg_dec<MISC_REGS>();
   if (warp == PROD_WARP) {
     // ------------------------------------------------------------- producer
     if (lane == 0) {
       Walk w(line, a);
-      int g = 0;
+      Slot<ST> r;
+      int issued = 0;
       bool ok = true;
       while (ok && w.next(a, nrb)) {
-        const int64_t kb = w.b * a.k.batch_stride + w.hk * a.k.head_stride;
-        const int64_t vb = w.b * a.v.batch_stride + w.hk * a.v.head_stride;
-        for (int t = 0; t < w.nt; ++t, ++g) {
-          const int st = g % ST, key0 = (w.t0 + t) * TK, nk = min(TK, w.kend - key0);
-          if (!(ok = wait1(&bar.empty[st], ((g / ST) & 1) ^ 1, fail))) break;
-          uint8_t* sb = ring + size_t(st) * C::STAGE;
+        int64_t kr = w.b * a.k.batch_stride + w.hk * a.k.head_stride + w.t0 * TK;  // row of the tile's first key
+        int64_t vr = w.b * a.v.batch_stride + w.hk * a.v.head_stride + w.t0 * TK;
+        int left = w.kend - w.t0 * TK;  // keys from the tile on
+#pragma unroll 1
+        for (int t = 0; t < w.nt; ++t, kr += TK, vr += TK, left -= TK) {
+          const int nk = min(TK, left);
+          if (!(ok = wait1(&bar.empty[r.i], r.par ^ 1, fail))) break;
+          uint8_t* sb = ring + r.i * C::STAGE;
+          uint64_t* full = &bar.full[r.i];
           uint32_t bytes = 2 * nk * C::KROW;
-          uintptr_t src[4];
-          uint32_t len[4];
           if constexpr (BITS != 0) {
+            // scales and biases: the 16-byte blocks that hold the tile's values
             const void* const arr[4] = {a.k.scales, a.k.biases, a.v.scales, a.v.biases};
+            uintptr_t src[4];
+            uint32_t len[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // the 16-byte blocks that hold the tile's values
-              const uintptr_t p = reinterpret_cast<uintptr_t>(arr[i]) + uintptr_t((i < 2 ? kb : vb) + key0) * C::SROW;
+            for (int i = 0; i < 4; ++i) {
+              const uintptr_t p = reinterpret_cast<uintptr_t>(arr[i]) + uintptr_t(i < 2 ? kr : vr) * C::SROW;
               src[i] = p & ~uintptr_t(15);
-              len[i] = uint32_t(((p + nk * C::SROW + 15) & ~uintptr_t(15)) - src[i]);
+              len[i] = (uint32_t(p & 15) + nk * C::SROW + 15) & ~15u;
               bytes += len[i];
             }
-          }
-          mbar_arrive_expect_tx(&bar.full[st], bytes);
-          bulk_g2s(sb + C::K_OFF, reinterpret_cast<const uint8_t*>(a.k.data) + (kb + key0) * C::KROW, nk * C::KROW,
-                   &bar.full[st]);
-          bulk_g2s(sb + C::V_OFF, reinterpret_cast<const uint8_t*>(a.v.data) + (vb + key0) * C::KROW, nk * C::KROW,
-                   &bar.full[st]);
-          if constexpr (BITS != 0) {
+            mbar_arrive_expect_tx(full, bytes);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              bulk_g2s(sb + C::S_OFF + i * C::SWIN, reinterpret_cast<const void*>(src[i]), len[i], &bar.full[st]);
+              bulk_g2s(sb + C::S_OFF + i * C::SWIN, reinterpret_cast<const void*>(src[i]), len[i], full);
+          } else {
+            mbar_arrive_expect_tx(full, bytes);
           }
+          bulk_g2s(sb + C::K_OFF, reinterpret_cast<const uint8_t*>(a.k.data) + kr * C::KROW, nk * C::KROW, full);
+          bulk_g2s(sb + C::V_OFF, reinterpret_cast<const uint8_t*>(a.v.data) + vr * C::KROW, nk * C::KROW, full);
+          ++issued;
+          r.next();
         }
       }
-      // the copies in flight land before the CTA may exit
-      for (int t = max(0, g - ST); t < g; ++t) (void)wait1(&bar.full[t % ST], (t / ST) & 1, fail);
+      // the copies in flight land before the CTA may exit: the last min(ST, issued) uses
+      Slot<ST> f;
+#pragma unroll 1
+      for (int i = 0; i < issued; ++i, f.next())
+        if (i >= issued - ST) (void)wait1(&bar.full[f.i], f.par, fail);
     }
-  } else if (warp == PREP_WARP) {
-    // --------------------------------------------------------------- scales
+  } else if (warp >= PREP_WARP) {
+    // ------------------------------------- scales, one warp per softmax stream
     if constexpr (BITS != 0) {
       Walk w(line, a);
+      Slot<ST> r;
       int g = 0;
       bool ok = true;
       while (ok && w.next(a, nrb)) {
-        int ev[2] = {-127, -127};  // running exponent of V in each stream
-        const int64_t kb = w.b * a.k.batch_stride + w.hk * a.k.head_stride;
-        const int64_t vb = w.b * a.v.batch_stride + w.hk * a.v.head_stride;
-        for (int t = 0; t < w.nt; ++t, ++g) {
-          const int st = g % ST, key0 = (w.t0 + t) * TK;
+        int ev = -127;  // running exponent of V
+        const uint32_t kb = uint32_t(w.b * a.k.batch_stride + w.hk * a.k.head_stride);  // only its low bits matter
+        const uint32_t vb = uint32_t(w.b * a.v.batch_stride + w.hk * a.v.head_stride);
+#pragma unroll 1
+        for (int t = 0; t < w.nt; ++t, ++g, r.next()) {
+          if ((g & 1) != warp - PREP_WARP) continue;
+          const int key0 = (w.t0 + t) * TK;
           unsigned long long vis = ~0ull;
           if (key0 + TK > w.n) vis = visible(seen_by_any(a, w.b, lane), key0, w.n, w.kend);
-          if (!(ok = waitw(&bar.full[st], (g / ST) & 1, fail))) break;
-          uint8_t* sb = ring + size_t(st) * C::STAGE;
+          if (!(ok = waitw(&bar.full[r.i], r.par, fail))) break;
+          uint8_t* sb = ring + r.i * C::STAGE;
           const void* const arr[4] = {a.k.scales, a.k.biases, a.v.scales, a.v.biases};
           float s[2][2 * G], b[2][2 * G], mx[2] = {0.f, 0.f};
 #pragma unroll
           for (int o = 0; o < 2; ++o) {  // K, V
-            const uint32_t at = uint32_t(o ? vb + key0 : kb + key0) * C::SROW;
+            const uint32_t at = ((o ? vb : kb) + key0) * C::SROW;
             const uint8_t* sp = sb + C::S_OFF + 2 * o * C::SWIN + ((uint32_t(reinterpret_cast<uintptr_t>(arr[2 * o])) + at) & 15);
             const uint8_t* bp = sb + C::S_OFF + (2 * o + 1) * C::SWIN +
                                 ((uint32_t(reinterpret_cast<uintptr_t>(arr[2 * o + 1])) + at) & 15);
@@ -525,12 +534,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             }
             mx[o] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[o])));
           }
-          const int ek = top_exp(mx[0]);
-          const int e2 = max(ev[g & 1], top_exp(mx[1]));
-          ev[g & 1] = e2;
+          const int ek = top_exp(mx[0], TOPQ);
+          const int e2 = ev = max(ev, top_exp(mx[1], TOPQ));
           if (lane == 0) {
-            s_kmul[g % EXPS] = pow2(ek);
-            s_ev[g % EXPS] = e2;
+            s_kmul[g & (EXPS - 1)] = pow2(ek);
+            s_ev[g & (EXPS - 1)] = e2;
           }
 #pragma unroll
           for (int o = 0; o < 2; ++o) {
@@ -538,181 +546,197 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             uint2* dst = reinterpret_cast<uint2*>(sb + C::H_OFF + o * TK * G * 8);
 #pragma unroll
             for (int i = 0; i < 2 * G; ++i) {
-              const float sf = s[o][i] * f, bfv = b[o][i] * f;
+              const float sf = s[o][i] * (f * (BITS == 8 ? 16777216.f : 1048576.f)), bfv = b[o][i] * f;
               dst[lane + 32 * i] = make_uint2(h2(sf, sf), h2(bfv, bfv));
             }
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.prep[st]);
+          if (lane == 0) mbar_arrive(&bar.prep[r.i]);
         }
       }
     }
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc(TK, false), id_o = idesc(D, true);
-      const uint32_t q_addr = smem_addr(qs), k_addr = smem_addr(kop), v_addr = smem_addr(vop);
-      Walk w(line, a);
-      int g0 = 0, seg = 0;
-      bool ok = true;
-      while (ok && w.next(a, nrb)) {
-        ok = wait1(&bar.qready, seg & 1, fail);
-        auto issue_s = [&](int g) -> bool {
-          const int j = g & 1, u = g >> 1, ob = g % NOP;
-          if (!wait1(&bar.kfull[ob], (g / NOP) & 1, fail)) return false;
-          // P of tile g - 4 sits in this buffer until its PV is done (a run's first two tiles: it is, and the phase is past)
-          if (g >= g0 + 2 && u >= 2 && !wait1(&bar.pvdone[j], (u - 2) & 1, fail)) return false;
-          tc_fence_after();
+    // the whole warp walks and waits, one elected lane issues
+    constexpr uint32_t id_s = idesc(TK, false), id_o = idesc(D, true);
+    const bool issuer = elect_one();
+    const uint64_t q_desc = sdesc(smem_addr(qs), 16), k_desc = sdesc(smem_addr(kop), 16),
+                   v_desc = sdesc(smem_addr(vop), TK * 128);
+    Walk w(line, a);
+    Slot<NOP> ks, vs;      // next K, V operand
+    int gs = 0, gp = 0;    // next tile's S, next tile's PV
+    uint32_t seg = 0;
+    bool ok = true;
+    // S of tile gs.  P of tile gs - 4 sits in its buffer until its PV is done; that of a run's
+    // first two tiles is (`fresh`), and its phase is past.
+    auto issue_s = [&](bool fresh) -> bool {
+      const int j = gs & 1, u = gs >> 1;
+      if (!waitw(&bar.kfull[ks.i], ks.par, fail)) return false;
+      if (!fresh && u >= 2 && !waitw(&bar.pvdone[j], u & 1, fail)) return false;
+      tc_fence_after();
+      if (issuer) {
+        const uint32_t d = tmem + S_COL + 64u * (2 * j + (u & 1));
+        const uint64_t kd = k_desc + uint32_t(ks.i * (C::OPER / 16));
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t blk = kk / 4, in = 2u * (kk % 4);
-            tc_mma_ss(tmem + S_COL + 64u * (2 * j + (u & 1)), sdesc(q_addr + blk * (ROWS * 128), 16) + in,
-                      sdesc(k_addr + ob * C::OPER + blk * (TK * 128), 16) + in, id_s, kk > 0 ? 1u : 0u);
-          }
-          tc_commit(&bar.sfull[2 * j + (u & 1)]);
-          tc_commit(&bar.kempty[ob]);
-          return true;
-        };
-        if (ok) ok = issue_s(g0);
-        if (ok && w.nt > 1) ok = issue_s(g0 + 1);
-        for (int t = 0; t < w.nt && ok; ++t) {
-          const int g = g0 + t, j = g & 1, u = g >> 1, ob = g % NOP;
-          if (t + 2 < w.nt && !(ok = issue_s(g + 2))) break;
-          if (!(ok = wait1(&bar.vfull[ob], (g / NOP) & 1, fail) && wait1(&bar.pfull[j], u & 1, fail))) break;
-          tc_fence_after();
+        for (int kk = 0; kk < D / 16; ++kk)
+          tc_mma_ss(d, q_desc + (kk / 4) * (ROWS * 128 / 16) + 2 * (kk % 4),
+                    kd + (kk / 4) * (TK * 128 / 16) + 2 * (kk % 4), id_s, kk > 0 ? 1u : 0u);
+        tc_commit(&bar.sfull[2 * j + (u & 1)]);
+        tc_commit(&bar.kempty[ks.i]);
+      }
+      __syncwarp();
+      ks.next();
+      ++gs;
+      return true;
+    };
+    while (ok && w.next(a, nrb)) {
+      ok = waitw(&bar.qready, seg & 1, fail);
+      ++seg;
+      // S runs two tiles ahead of PV
+#pragma unroll 1
+      for (int t = -2; t < w.nt && ok; ++t) {
+        if (t + 2 < w.nt && !(ok = issue_s(t < 0))) break;
+        if (t < 0) continue;
+        const int j = gp & 1, u = gp >> 1;
+        if (!(ok = waitw(&bar.vfull[vs.i], vs.par, fail) && waitw(&bar.pfull[j], u & 1, fail))) break;
+        tc_fence_after();
+        if (issuer) {
+          const uint32_t d = tmem + O_COL + 128u * j, p = tmem + S_COL + 64u * (2 * j + (u & 1));
+          const uint64_t vd = v_desc + uint32_t(vs.i * (C::OPER / 16));
 #pragma unroll
           for (int kk = 0; kk < TK / 16; ++kk)
-            tc_mma_ts(tmem + O_COL + 128u * j, tmem + S_COL + 64u * (2 * j + (u & 1)) + 8u * kk,
-                      sdesc(v_addr + ob * C::OPER + kk * 2048, TK * 128), id_o, (t > 1 || kk > 0) ? 1u : 0u);
+            tc_mma_ts(d, p + 8u * kk, vd + kk * (2048 / 16), id_o, (t > 1 || kk > 0) ? 1u : 0u);
           tc_commit(&bar.pvdone[j]);
-          tc_commit(&bar.vempty[ob]);
+          tc_commit(&bar.vempty[vs.i]);
         }
-        g0 += w.nt;
-        ++seg;
+        __syncwarp();
+        vs.next();
+        ++gp;
       }
-      // every MMA issued has completed before TMEM may be freed
-      tc_commit(&bar.idle);
-      (void)wait1(&bar.idle, 0, fail);
     }
-  } else if (warp >= SMX_WARPS) {
+    // every MMA issued has completed before TMEM may be freed
+    if (issuer) tc_commit(&bar.idle);
+    __syncwarp();
+    (void)waitw(&bar.idle, 0, fail);
+  } else if (warp >= SMX_WARPS && warp < MMA_WARP) {
     // ------------------------------------------------------------ conversion
-    const int d = tid - SMX_WARPS * 32;
-    constexpr int PIECES = D / 16, PER = TK * PIECES / (DQ_WARPS * 32);  // 16-dim pieces of a row; per thread and operand
+    // A thread takes dims 16 c .. 16 c + 15 of every KSTEP-th key of a tile.  The 8
+    // lanes of a shared-memory phase must read 8 different 16-byte columns and
+    // write 8 different (chunk ^ key & 7): with two groups they hold the pieces 0-3 of
+    // one key and 4-7 of its neighbour (8/4-bit rows), or all pieces of
+    // one key with the halves of 4-7 in the other order (bf16 rows of 256 bytes).
+    setmaxnreg_dec<DQ_REGS>();
+    const int o = warp >= SMX_WARPS + DQ_WARPS;  // K, V
+    const int d = tid - (SMX_WARPS + o * DQ_WARPS) * 32;
+    constexpr int PIECES = D / 16, KSTEP = DQ_WARPS * 32 / PIECES, PER = TK / KSTEP;
+    const int c = d % PIECES;
+    const int key = G == 2 && BITS != 0 ? 2 * (d >> 4) + (((d >> 2) ^ (d >> 3)) & 1) : d / PIECES;
+    const int swap = G == 2 && BITS == 0 ? c >> 2 : 0;  // order of the two 8-dim chunks
+    uint32_t to[2];  // where they go; key & 7 is the same for all of a thread's keys
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int ch = 2 * c + (hh ^ swap);
+      to[hh] = (ch >> 3) * (TK * 128) + sw128(key, ch & 7);
+    }
+    static_assert(KSTEP % 8 == 0, "a thread's keys share key & 7");
+    uint64_t* const fullb = o ? bar.vfull : bar.kfull;
+    uint64_t* const emptyb = o ? bar.vempty : bar.kempty;
+    uint8_t* const oper = o ? vop : kop;
+    const uint32_t from0 = (o ? C::V_OFF : C::K_OFF) + key * C::KROW + c * (BITS ? 2 * BITS : 32);
     Walk w(line, a);
+    Slot<ST> r;
+    Slot<NOP> q;
     int g = 0;
     bool ok = true;
     while (ok && w.next(a, nrb)) {
-      int ev[2] = {-127, -127};
+      int ev0 = -127, ev1 = -127;
+#pragma unroll 1
       for (int t = 0; t < w.nt; ++t, ++g) {
-        const int st = g % ST, ob = g % NOP;
-        const uint8_t* sb = ring + size_t(st) * C::STAGE;
-        unsigned long long vis = ~0ull;
+        const uint8_t* sb = ring + r.i * C::STAGE;
+        const uint8_t* src = sb + from0;
+        uint8_t* dst = oper + q.i * C::OPER;
         if constexpr (BITS == 0) {
           const int key0 = (w.t0 + t) * TK;
-          if (key0 + TK > w.n) vis = visible(seen_by_any(a, w.b, lane), key0, w.n, w.kend);
-        } else {
-          if (!(ok = waitw(&bar.prep[st], (g / ST) & 1, fail))) break;
-        }
-        if (!(ok = waitw(&bar.full[st], (g / ST) & 1, fail))) break;
-        // bf16 caches: both operands' values and largest exponents first (the softmax reads them with S)
-        uint4 x[BITS == 0 ? 2 : 1][PER][2];
-        float scale16[2];
-        if constexpr (BITS == 0) {
+          unsigned long long vis = ~0ull;
+          if (key0 + TK > w.n) vis = visible(seen_by_any(a, w.b, lane), key0, w.n, w.kend) >> key;
+          else vis >>= key;
+          if (!(ok = waitw(&bar.full[r.i], r.par, fail))) break;
+          uint4 x[PER][2];
+          uint32_t mx = 0;
 #pragma unroll
-          for (int o = 0; o < 2; ++o) {
-            const uint8_t* src = sb + (o ? C::V_OFF : C::K_OFF);
-            uint32_t mx = 0;
+          for (int i = 0; i < PER; ++i) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const int e = d + i * DQ_WARPS * 32, key = e / PIECES, c = e % PIECES;
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                // halves of the row's upper group in the other order: the 8 lanes of a phase hit 8 bank groups
-                const int h = G == 2 ? hh ^ (c >> 2) : hh;
-                const uint4 y = ((vis >> key) & 1) ? *reinterpret_cast<const uint4*>(src + key * C::KROW + (2 * c + h) * 16)
-                                                   : make_uint4(0, 0, 0, 0);
-                x[o][i][hh] = y;
-                mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(y.x & 0x7FFF7FFFu, y.y & 0x7FFF7FFFu),
-                                           __vmaxu2(y.z & 0x7FFF7FFFu, y.w & 0x7FFF7FFFu)));
-              }
-            }
-            mx = __reduce_max_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16));
-            if (lane == 0) s_dqmax[g & 1][o][warp - SMX_WARPS] = __uint_as_float(mx << 16);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.dqmax);
-          if (!(ok = waitw(&bar.dqmax, g & 1, fail))) break;
-          float m[2] = {0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < DQ_WARPS; ++i) {
-            m[0] = fmaxf(m[0], s_dqmax[g & 1][0][i]);
-            m[1] = fmaxf(m[1], s_dqmax[g & 1][1][i]);
-          }
-          const int ek = top_exp(m[0]);
-          ev[g & 1] = max(ev[g & 1], top_exp(m[1]));
-          if (d == 0) {
-            s_kmul[g % EXPS] = pow2(ek);
-            s_ev[g % EXPS] = ev[g & 1];
-          }
-          scale16[0] = pow2(-ek);
-          scale16[1] = pow2(-ev[g & 1]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.empty[st]);
-        }
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {  // K, V
-          uint64_t* fullb = o ? bar.vfull : bar.kfull;
-          uint64_t* emptyb = o ? bar.vempty : bar.kempty;
-          uint8_t* dst = (o ? vop : kop) + ob * C::OPER;
-          const uint8_t* src = sb + (o ? C::V_OFF : C::K_OFF);
-          if constexpr (BITS == 0) {
-            if (!(ok = waitw(&emptyb[ob], ((g / NOP) & 1) ^ 1, fail))) break;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const int e = d + i * DQ_WARPS * 32, key = e / PIECES, c = e % PIECES;
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const int ch = 2 * c + (G == 2 ? hh ^ (c >> 2) : hh);
-                *reinterpret_cast<uint4*>(dst + (ch >> 3) * (TK * 128) + sw128(key, ch & 7)) = conv16(x[o][i][hh], scale16[o]);
-              }
-            }
-          } else {
-            const uint2* sc = reinterpret_cast<const uint2*>(sb + C::H_OFF + o * TK * G * 8);
-            if (!(ok = waitw(&emptyb[ob], ((g / NOP) & 1) ^ 1, fail))) break;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const int e = d + i * DQ_WARPS * 32, key = e / PIECES, c = e % PIECES;
-              const uint2 sbv = sc[key * G + (G == 2 ? c >> 2 : 0)];
-              uint4 v[2];
-              if constexpr (BITS == 8) {
-                const uint4 x = *reinterpret_cast<const uint4*>(src + key * C::KROW + c * 16);
-                v[0] = conv8(make_uint2(x.x, x.y), sbv.x, sbv.y);
-                v[1] = conv8(make_uint2(x.z, x.w), sbv.x, sbv.y);
-              } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(src + key * C::KROW + c * 8);
-                v[0] = conv4(x.x, sbv.x, sbv.y);
-                v[1] = conv4(x.y, sbv.x, sbv.y);
-              }
-              const bool sw = G == 2 && (c >> 2);  // upper group: halves in the other order (bank groups)
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const int ch = 2 * c + (sw ? hh ^ 1 : hh);
-                *reinterpret_cast<uint4*>(dst + (ch >> 3) * (TK * 128) + sw128(key, ch & 7)) = sw ? v[hh ^ 1] : v[hh];
-              }
+            for (int hh = 0; hh < 2; ++hh) {
+              const uint4 y = ((vis >> (i * KSTEP)) & 1)
+                                  ? *reinterpret_cast<const uint4*>(src + i * (KSTEP * C::KROW) + 16 * (hh ^ swap))
+                                  : make_uint4(0, 0, 0, 0);
+              x[i][hh] = y;
+              mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(y.x & 0x7FFF7FFFu, y.y & 0x7FFF7FFFu),
+                                         __vmaxu2(y.z & 0x7FFF7FFFu, y.w & 0x7FFF7FFFu)));
             }
           }
-          fence_async_smem();
-          __syncwarp();
+          mx = __reduce_max_sync(0xffffffffu, max(mx & 0xFFFFu, mx >> 16));
           if (lane == 0) {
-            mbar_arrive(&fullb[ob]);
-            if (BITS != 0 && o) mbar_arrive(&bar.empty[st]);
+            s_dqmax[g & 1][o][warp & (DQ_WARPS - 1)] = __uint_as_float(mx << 16);
+            mbar_arrive(&bar.dqmax[o]);
+            mbar_arrive(&bar.empty[r.i]);
+          }
+          if (!(ok = waitw(&bar.dqmax[o], g & 1, fail))) break;
+          float m = 0.f;
+#pragma unroll
+          for (int i = 0; i < DQ_WARPS; ++i) m = fmaxf(m, s_dqmax[g & 1][o][i]);
+          int e = top_exp(m, TOP16);
+          if (o) {
+            e = max(ev0, e);
+            ev0 = ev1;
+            ev1 = e;
+          }
+          if (d == 0) {
+            if (o) s_ev[g & (EXPS - 1)] = e;
+            else s_kmul[g & (EXPS - 1)] = pow2(e);
+          }
+          const float f = pow2(-e);
+          if (!(ok = waitw(&emptyb[q.i], q.par ^ 1, fail))) break;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            *reinterpret_cast<uint4*>(dst + to[0] + i * (KSTEP * 128)) = conv16(x[i][0], f);
+            *reinterpret_cast<uint4*>(dst + to[1] + i * (KSTEP * 128)) = conv16(x[i][1], f);
+          }
+        } else {
+          if (!(ok = waitw(&bar.prep[r.i], r.par, fail) && waitw(&bar.full[r.i], r.par, fail) &&
+                     waitw(&emptyb[q.i], q.par ^ 1, fail)))
+            break;
+          const uint2* sc = reinterpret_cast<const uint2*>(sb + C::H_OFF + o * TK * G * 8) + key * G + (G == 2 ? c >> 2 : 0);
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const uint2 f = sc[i * KSTEP * G];
+            uint4 v[2];
+            if constexpr (BITS == 8) {
+              const uint4 y = *reinterpret_cast<const uint4*>(src + i * (KSTEP * C::KROW));
+              v[0] = conv8(make_uint2(y.x, y.y), f.x, f.y);
+              v[1] = conv8(make_uint2(y.z, y.w), f.x, f.y);
+            } else {
+              const uint2 y = *reinterpret_cast<const uint2*>(src + i * (KSTEP * C::KROW));
+              v[0] = conv4(y.x, f.x, f.y);
+              v[1] = conv4(y.y, f.x, f.y);
+            }
+            *reinterpret_cast<uint4*>(dst + to[0] + i * (KSTEP * 128)) = v[0];
+            *reinterpret_cast<uint4*>(dst + to[1] + i * (KSTEP * 128)) = v[1];
           }
         }
-        if (!ok) break;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&fullb[q.i]);
+          if (BITS != 0) mbar_arrive(&bar.empty[r.i]);
+        }
+        r.next();
+        q.next();
       }
     }
-  } else {
+  } else if (warp < SMX_WARPS) {
     // ---------------------------------------------------------------- softmax
+    setmaxnreg_inc<SMX_REGS>();
     const int j = warp >> 2, r = tid & 127;      // stream, lane of tensor memory
     const uint32_t lrow = uint32_t(32 * (warp & 3)) << 16;
     Walk w(line, a);
@@ -738,7 +762,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
         for (int i = 0; i < D / 8; ++i)
           mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu),
                                      __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
-        const int eq = top_exp(__uint_as_float(max(mx & 0xFFFFu, mx >> 16) << 16));
+        const int eq = top_exp(__uint_as_float(max(mx & 0xFFFFu, mx >> 16) << 16), TOP16);
         const float f = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
         c_row = fmaxf(fabsf(a.scale) * LOG2E * pow2(eq), 1e-37f);
 #pragma unroll
@@ -757,6 +781,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
       }
       Row st{-INFINITY, 0.f, 0};
       int last = -1;  // this stream's last tile
+#pragma unroll 1
       for (int g = g0 + ((g0 & 1) ^ j); g < g0 + w.nt && ok; g += 2) {
         const int u = g >> 1, buf = 2 * j + (u & 1), key0 = (w.t0 + g - g0) * TK;
         if (!(ok = waitw(&bar.sfull[buf], (u >> 1) & 1, fail))) break;
@@ -764,16 +789,25 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
           tc_fence_after();
           const bool edge = key0 + TK > w.n;
           const unsigned long long vis = edge ? visible(word, key0, w.n, w.kend) : 0ull;
-          const float c = c_row * s_kmul[g % EXPS];
-          const int ev = s_ev[g % EXPS];
-          const uint32_t sa = tmem + lrow + S_COL + 64u * buf, oa = tmem + lrow + O_COL + 128u * j;
-          if (rep == 1)
-            ok = softmax_tile<64, D>(st, sa, oa, 0, c, ev, edge, vis, last < 0, &bar.pvdone[j], (u - 1) & 1, fail);
-          else if (rep == 2)
-            ok = softmax_tile<32, D>(st, sa, oa, off, c, ev, edge, vis, last < 0, &bar.pvdone[j], (u - 1) & 1, fail);
-          else
-            ok = softmax_tile<16, D>(st, sa, oa, off, c, ev, edge, vis, last < 0, &bar.pvdone[j], (u - 1) & 1, fail);
-          if (!ok) break;
+          const float c = c_row * s_kmul[g & (EXPS - 1)];
+          const uint32_t sa = tmem + lrow + S_COL + 64u * buf;
+          float corr = rep == 1   ? softmax_tile<64>(st, sa, 0, c, edge, vis)
+                       : rep == 2 ? softmax_tile<32>(st, sa, off, c, edge, vis)
+                                  : softmax_tile<16>(st, sa, off, c, edge, vis);
+          // V's exponent in this stream; for bf16 caches it is there once the tile's V is (whose
+          // buffer cannot be refilled before this P is used: its phase stands still)
+          if (BITS == 0 && !(ok = waitw(&bar.vfull[g % NOP], (g / NOP) & 1, fail))) break;
+          const int ev = s_ev[g & (EXPS - 1)];
+          if (last >= 0) {
+            if (ev != st.ev) corr *= pow2(max(st.ev - ev, -126));
+            if (__any_sync(0xffffffffu, corr != 1.f)) {
+              if (!(ok = waitw(&bar.pvdone[j], (u - 1) & 1, fail))) break;
+              tc_fence_after();
+              scale_o<D>(tmem + lrow + O_COL + 128u * j, corr);
+            }
+          }
+          st.ev = ev;
+          tmem_st_wait();
           tc_fence_before();
         }
         __syncwarp();
@@ -792,12 +826,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
         const float M = fmaxf(x.m, y.m);
         const float wx = x.m == -INFINITY ? 0.f : ex2(x.m - M), wy = y.m == -INFINITY ? 0.f : ex2(y.m - M);
         const float l = x.l * wx + y.l * wy;
-        const bool direct = w.whole && rep == 1;
+        const bool direct = w.whole() && rep == 1;
         const float inv = direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
         const float fx = wx * pow2(x.ev) * inv, fy = wy * pow2(y.ev) * inv;
         const size_t slot = size_t(cta_slot + w.pair) * ROWS + r;
         bf16* out = a.out + w.b * a.o_sb + h * a.o_sh + qi * a.o_sl;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < D / 2; i += 16) {  // stream j's warps write half of the dims
           const int d0 = j * (D / 2) + i;
           float o0[16], o1[16];
@@ -858,27 +892,18 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const TreeAt
   const int grp = a.Hq / a.Hkv, R = a.L * grp, pairs = a.Hkv * nrb;
   const int row = blockIdx.x % R, hk = blockIdx.x / R % a.Hkv, b = blockIdx.x / R / a.Hkv;
   const int rb = row / ROWS, lr = row % ROWS, rep = repeats(min(ROWS, R - rb * ROWS)), per = ROWS / rep;
-  long long total, base = 0;
-  {
-    // tiles before sequence b, and in all
-    long long before = 0, all = 0;
-    for (int i = lane; i < a.B; i += 32) {
-      const long long t = (long long)seq_tiles(a, i) * pairs;
-      all += t;
-      if (i < b) before += t;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      all += __shfl_xor_sync(0xffffffffu, all, o);
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    total = all;
-    base = before;
+  int total = 0, base = 0;  // tiles of all sequences, and of those before b
+  for (int i = lane; i < a.B; i += 32) {
+    const int t = seq_tiles(a, i) * pairs;
+    total += t;
+    if (i < b) base += t;
   }
-  const int tiles = seq_tiles(a, b), p = hk * nrb + rb, np = parts(a, total, ctas);
-  const long long t0 = base + (long long)p * tiles, t1 = t0 + tiles - 1;
+  total = __reduce_add_sync(0xffffffffu, total);
+  base = __reduce_add_sync(0xffffffffu, base);
+  const int tiles = seq_tiles(a, b), p = hk * nrb + rb, np = parts(total, ctas);
+  const int t0 = base + p * tiles, t1 = t0 + tiles - 1;
   // part c holds tile t: total * c / np <= t
-  const int c0 = (int)(((t0 + 1) * np - 1) / total), c1 = (int)(((t1 + 1) * np - 1) / total);
+  const int c0 = (int)(((t0 + 1LL) * np - 1) / total), c1 = (int)(((t1 + 1LL) * np - 1) / total);
   if (c0 == c1 && rep == 1) return;  // written by the attention kernel
   const int n = (c1 - c0 + 1) * rep;
   const size_t slot0 = size_t(c0 + b * pairs + p) * ROWS + lr;

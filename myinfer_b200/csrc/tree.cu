@@ -210,6 +210,9 @@ int m5::tree_attn_check(const TreeAttnArgs& a) {
   M5_CHECK_ARG(!a.bits || (a.k.scales && a.k.biases && a.v.scales && a.v.biases),
                "m5_tree_attention: packed K/V need scales and biases");
   M5_CHECK_ARG(a.capacity + kTreeMax < (1LL << 31), "m5_tree_attention: capacity must stay below 2^31 rows");
+  const int64_t blocks = (int64_t(a.L) * (a.Hq / a.Hkv) + 127) / 128;
+  M5_CHECK_ARG(int64_t(a.B) * a.Hkv < (1LL << 31) / blocks / ((a.capacity + 63) / 64),
+               "m5_tree_attention: more than 2^31 tiles of 128 rows and 64 keys");
   M5_CHECK_ARG((reinterpret_cast<uintptr_t>(a.k.data) | reinterpret_cast<uintptr_t>(a.v.data)) % 16 == 0,
                "m5_tree_attention: K/V rows must be 16-byte aligned");
   M5_CHECK_ARG((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) % 16 == 0 &&
