@@ -56,7 +56,6 @@ constexpr int THREADS = (PREP_WARP + 2) * 32;
 // registers per thread after setmaxnreg: 2 + 2 + 1 warpgroups out of 640 x 96 at launch
 constexpr int SMX_REGS = 136, DQ_REGS = 72, MISC_REGS = 56;
 static_assert(256 * SMX_REGS + 256 * DQ_REGS + 128 * MISC_REGS <= 640 * 96, "register split");
-constexpr int NOP = 3;      // converted K and V tiles held
 constexpr int EXPS = 32;    // tile exponents held: more than the tiles between conversion and softmax
 constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -68,7 +67,8 @@ constexpr float LAZY = 8.f; // log2 growth of a row's maximum that is left in p
 constexpr int TOP16 = 7, TOPQ = -3;
 constexpr int MIN_TILES = 2;  // per CTA: one per stream
 
-template <int BITS, int D>
+// TWO: a CTA holds two blocks of 128 rows, one per softmax stream; else one
+template <int BITS, int D, bool TWO>
 struct Cfg {
   static constexpr int G = D / 64;                              // scale groups
   static constexpr int KROW = BITS ? D * BITS / 8 : 2 * D;      // bytes of a packed row
@@ -79,19 +79,23 @@ struct Cfg {
   static constexpr int H_OFF = S_OFF + 4 * SWIN;                // fp16 (s, s), (b, b) per key and group, K then V
   static constexpr int STAGE = (H_OFF + (BITS ? 2 * TK * G * 8 : 0) + 127) / 128 * 128;
   static constexpr int OPER = TK * D * 2;                       // a converted tile
-  static constexpr int QBYTES = ROWS * D * 2;
+  static constexpr int NOP = TWO && BITS == 0 && D == 128 ? 2 : 3;  // converted K and V tiles held
+  static constexpr int BLOCKS = TWO ? 2 : 1;
+  static constexpr int QBLOCK = ROWS * D * 2, QBYTES = BLOCKS * QBLOCK;
   static constexpr int FIXED = QBYTES + 2 * NOP * OPER + 1024 + 1024;  // + alignment, barriers
   static constexpr int ST = (227 * 1024 - 4096 - FIXED) / STAGE < 8 ? (227 * 1024 - 4096 - FIXED) / STAGE : 8;
   static constexpr int SMEM = FIXED + ST * STAGE;
 };
 
 // Barriers, in the order of the array.
-template <int ST>
+template <int ST, int NOP>
 struct Bars {
   uint64_t full[ST], empty[ST], prep[ST];
   uint64_t kfull[NOP], kempty[NOP], vfull[NOP], vempty[NOP];
-  uint64_t sfull[4];   // [stream][buffer]
-  uint64_t pfull[2], pvdone[2];
+  // [stream][buffer].  P and PV need one per buffer too.  S of the next tile is there ahead, so a
+  // warp may hand over that tile's P before its neighbours have handed over this one's; and a
+  // stream may be two PVs ahead of the last finished one, which one phase bit cannot tell.
+  uint64_t sfull[4], pfull[4], pvdone[4];
   uint64_t qready, idle;
   uint64_t dqmax[2];   // [K, V] bf16 caches: the conversion warps' maxima of a tile are in shared memory
 };
@@ -157,9 +161,28 @@ __device__ __forceinline__ bool wait1(uint64_t* bar, uint32_t par, volatile int*
   atomicExch(&g_attn_tree_err, M5_DEV_ERR_WAIT_TIMEOUT);
   return false;
 }
-// by a warp: every lane polls, the result is the same for all
-__device__ __forceinline__ bool waitw(uint64_t* bar, uint32_t par, volatile int* fail) {
-  return __all_sync(0xffffffffu, wait1(bar, par, fail));
+// Waits by a warp, with one answer for all lanes.  A poll takes 80 cycles even when the phase is
+// complete (110 with a suspend-time hint, 120 when one lane polls for the others), so what
+// is needed together is polled together.
+struct Ph {
+  uint64_t* bar;
+  uint32_t par;
+};
+__device__ __forceinline__ bool waitw(volatile int* fail, Ph a) {
+  if (__all_sync(0xffffffffu, mbar_try_wait_fast(a.bar, a.par))) return true;
+  return __all_sync(0xffffffffu, wait1(a.bar, a.par, fail));
+}
+__device__ __forceinline__ bool waitw(volatile int* fail, Ph a, Ph b) {
+  const bool x = mbar_try_wait_fast(a.bar, a.par), y = mbar_try_wait_fast(b.bar, b.par);
+  if (__all_sync(0xffffffffu, x && y)) return true;
+  return __all_sync(0xffffffffu, wait1(a.bar, a.par, fail) && wait1(b.bar, b.par, fail));
+}
+__device__ __forceinline__ bool waitw(volatile int* fail, Ph a, Ph b, Ph c) {
+  const bool x = mbar_try_wait_fast(a.bar, a.par), y = mbar_try_wait_fast(b.bar, b.par),
+             z = mbar_try_wait_fast(c.bar, c.par);
+  if (__all_sync(0xffffffffu, x && y && z)) return true;
+  return __all_sync(0xffffffffu,
+                    wait1(a.bar, a.par, fail) && wait1(b.bar, b.par, fail) && wait1(c.bar, c.par, fail));
 }
 
 // A slot of a ring of N buffers and the parity of its current use.
@@ -379,19 +402,19 @@ __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, 
   return corr;
 }
 
-template <int BITS, int D>
+template <int BITS, int D, bool TWO>
 __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArgs a, const int nrb, float* part_o,
                                                                float2* part_ml) {
-  using C = Cfg<BITS, D>;
-  constexpr int ST = C::ST, G = C::G;
+  using C = Cfg<BITS, D, TWO>;
+  constexpr int ST = C::ST, G = C::G, NOP = C::NOP;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* qs = base;                         // [G][128 rows][128 bytes]
+  uint8_t* qs = base;                         // [blocks][G][128 rows][128 bytes]
   uint8_t* kop = qs + C::QBYTES;              // [NOP][G][64 keys][128 bytes]
   uint8_t* vop = kop + NOP * C::OPER;
   uint8_t* ring = vop + NOP * C::OPER;
-  Bars<ST>& bar = *reinterpret_cast<Bars<ST>*>(ring + ST * C::STAGE);
-  static_assert(sizeof(Bars<ST>) <= 1024, "barriers");
+  Bars<ST, NOP>& bar = *reinterpret_cast<Bars<ST, NOP>*>(ring + ST * C::STAGE);
+  static_assert(sizeof(Bars<ST, NOP>) <= 1024, "barriers");
   __shared__ Row s_row[2][ROWS];
   __shared__ float s_kmul[EXPS];
   __shared__ int s_ev[EXPS];
@@ -417,8 +440,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
       mbar_init(&bar.kempty[i], 1);
       mbar_init(&bar.vempty[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&bar.sfull[i], 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bar.sfull[i], 1);
       mbar_init(&bar.pfull[i], SMX_WARPS / 2);
       mbar_init(&bar.pvdone[i], 1);
     }
@@ -445,7 +468,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const Line line = s_line;
-  const int cta_slot = blockIdx.x;
 
   if (warp >= MMA_WARP) setmaxnreg_dec<MISC_REGS>();
   if (warp == PROD_WARP) {
@@ -498,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
         if (i >= issued - ST) (void)wait1(&bar.full[f.i], f.par, fail);
     }
   } else if (warp >= PREP_WARP) {
-    // ------------------------------------- scales, one warp per softmax stream
+    // --------- scales: one warp per stream, or one for tiles both streams take
     if constexpr (BITS != 0) {
       Walk w(line, a);
       Slot<ST> r;
@@ -510,11 +532,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
         const uint32_t vb = uint32_t(w.b * a.v.batch_stride + w.hk * a.v.head_stride);
 #pragma unroll 1
         for (int t = 0; t < w.nt; ++t, ++g, r.next()) {
-          if ((g & 1) != warp - PREP_WARP) continue;
+          if (TWO ? warp != PREP_WARP : (g & 1) != warp - PREP_WARP) continue;  // V's exponent belongs to a stream
           const int key0 = (w.t0 + t) * TK;
           unsigned long long vis = ~0ull;
           if (key0 + TK > w.n) vis = visible(seen_by_any(a, w.b, lane), key0, w.n, w.kend);
-          if (!(ok = waitw(&bar.full[r.i], r.par, fail))) break;
+          if (!(ok = waitw(fail, {&bar.full[r.i], r.par}))) break;
           uint8_t* sb = ring + r.i * C::STAGE;
           const void* const arr[4] = {a.k.scales, a.k.biases, a.v.scales, a.v.biases};
           float s[2][2 * G], b[2][2 * G], mx[2] = {0.f, 0.f};
@@ -562,62 +584,96 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     const bool issuer = elect_one();
     const uint64_t q_desc = sdesc(smem_addr(qs), 16), k_desc = sdesc(smem_addr(kop), 16),
                    v_desc = sdesc(smem_addr(vop), TK * 128);
+    // Tiles go to the streams in turn, or (TWO) each to both: u counts a stream's tiles.  S runs
+    // ahead of PV so that a softmax warp finds its next S in place when it has handed over P,
+    // and each PV is followed by an S that waits for nothing recent:
+    //   one block   PV(t), S(t + 3)                            (tiles t, t + 3 of different streams)
+    //   TWO         PV_0(t), S_1(t + 1), PV_1(t), S_0(t + 2)
     Walk w(line, a);
-    Slot<NOP> ks, vs;      // next K, V operand
-    int gs = 0, gp = 0;    // next tile's S, next tile's PV
-    uint32_t seg = 0;
-    bool ok = true;
-    // S of tile gs.  P of tile gs - 4 sits in its buffer until its PV is done; that of a run's
-    // first two tiles is (`fresh`), and its phase is past.
-    auto issue_s = [&](bool fresh) -> bool {
-      const int j = gs & 1, u = gs >> 1;
-      if (!waitw(&bar.kfull[ks.i], ks.par, fail)) return false;
-      if (!fresh && u >= 2 && !waitw(&bar.pvdone[j], u & 1, fail)) return false;
-      tc_fence_after();
+    auto s_mma = [&](int j, int u, int slot, bool last_use) {
       if (issuer) {
         const uint32_t d = tmem + S_COL + 64u * (2 * j + (u & 1));
-        const uint64_t kd = k_desc + uint32_t(ks.i * (C::OPER / 16));
+        const uint64_t qd = q_desc + (TWO ? j * (C::QBLOCK / 16) : 0), kd = k_desc + uint32_t(slot * (C::OPER / 16));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          tc_mma_ss(d, q_desc + (kk / 4) * (ROWS * 128 / 16) + 2 * (kk % 4),
+          tc_mma_ss(d, qd + (kk / 4) * (ROWS * 128 / 16) + 2 * (kk % 4),
                     kd + (kk / 4) * (TK * 128 / 16) + 2 * (kk % 4), id_s, kk > 0 ? 1u : 0u);
         tc_commit(&bar.sfull[2 * j + (u & 1)]);
-        tc_commit(&bar.kempty[ks.i]);
+        if (last_use) tc_commit(&bar.kempty[slot]);
       }
       __syncwarp();
-      ks.next();
-      ++gs;
-      return true;
     };
-    while (ok && w.next(a, nrb)) {
-      ok = waitw(&bar.qready, seg & 1, fail);
-      ++seg;
-      // S runs two tiles ahead of PV
-#pragma unroll 1
-      for (int t = -2; t < w.nt && ok; ++t) {
-        if (t + 2 < w.nt && !(ok = issue_s(t < 0))) break;
-        if (t < 0) continue;
-        const int j = gp & 1, u = gp >> 1;
-        if (!(ok = waitw(&bar.vfull[vs.i], vs.par, fail) && waitw(&bar.pfull[j], u & 1, fail))) break;
-        tc_fence_after();
-        if (issuer) {
-          const uint32_t d = tmem + O_COL + 128u * j, p = tmem + S_COL + 64u * (2 * j + (u & 1));
-          const uint64_t vd = v_desc + uint32_t(vs.i * (C::OPER / 16));
+    auto pv_mma = [&](int j, int u, int slot, bool first, bool last_use) {
+      if (issuer) {
+        const uint32_t d = tmem + O_COL + 128u * j, p = tmem + S_COL + 64u * (2 * j + (u & 1));
+        const uint64_t vd = v_desc + uint32_t(slot * (C::OPER / 16));
 #pragma unroll
-          for (int kk = 0; kk < TK / 16; ++kk)
-            tc_mma_ts(d, p + 8u * kk, vd + kk * (2048 / 16), id_o, (t > 1 || kk > 0) ? 1u : 0u);
-          tc_commit(&bar.pvdone[j]);
-          tc_commit(&bar.vempty[vs.i]);
-        }
-        __syncwarp();
-        vs.next();
-        ++gp;
+        for (int kk = 0; kk < TK / 16; ++kk)
+          tc_mma_ts(d, p + 8u * kk, vd + kk * (2048 / 16), id_o, (kk > 0 || !first) ? 1u : 0u);
+        tc_commit(&bar.pvdone[2 * j + (u & 1)]);
+        if (last_use) tc_commit(&bar.vempty[slot]);
       }
+      __syncwarp();
+    };
+    // the phase of PV(u - 2), whose P sits in the buffer S(u) goes to (u < 2: complete at once)
+    auto free_s = [&](int j, int u) { return Ph{&bar.pvdone[2 * j + (u & 1)], uint32_t((u >> 1) + 1) & 1}; };
+    auto p_of = [&](int j, int u) { return Ph{&bar.pfull[2 * j + (u & 1)], uint32_t(u >> 1) & 1}; };
+    Slot<NOP> ks, k1, vs;  // next K (TWO: of stream 0, of stream 1), next V
+    int g0 = 0;            // tiles before the run
+    uint32_t seg = 0;
+    bool ok = true;
+    while (ok && w.next(a, nrb)) {
+      ok = waitw(fail, {&bar.qready, seg & 1});
+      ++seg;
+      constexpr int AHEAD = TWO ? 2 : 3;
+#pragma unroll 1
+      for (int t = -AHEAD; t < w.nt && ok; ++t) {
+        const int g = g0 + t;
+        if constexpr (TWO) {
+          if (t >= 0) {
+            if (!(ok = waitw(fail, {&bar.vfull[vs.i], vs.par}, p_of(0, g)))) break;
+            tc_fence_after();
+            pv_mma(0, g, vs.i, t == 0, false);
+          }
+          if (t >= -1 && t + 1 < w.nt) {  // its K is there: S_0(t + 1) has used it
+            if (!(ok = waitw(fail, free_s(1, g + 1)))) break;
+            tc_fence_after();
+            s_mma(1, g + 1, k1.i, true);
+            k1.next();
+          }
+          if (t >= 0) {
+            if (!(ok = waitw(fail, p_of(1, g)))) break;
+            tc_fence_after();
+            pv_mma(1, g, vs.i, t == 0, true);
+            vs.next();
+          }
+          if (t + 2 < w.nt) {
+            if (!(ok = waitw(fail, {&bar.kfull[ks.i], ks.par}, free_s(0, g + 2)))) break;
+            tc_fence_after();
+            s_mma(0, g + 2, ks.i, false);
+            ks.next();
+          }
+        } else {
+          if (t >= 0) {
+            if (!(ok = waitw(fail, {&bar.vfull[vs.i], vs.par}, p_of(g & 1, g >> 1)))) break;
+            tc_fence_after();
+            pv_mma(g & 1, g >> 1, vs.i, t < 2, true);
+            vs.next();
+          }
+          if (t + 3 < w.nt) {
+            if (!(ok = waitw(fail, {&bar.kfull[ks.i], ks.par}, free_s((g + 3) & 1, (g + 3) >> 1)))) break;
+            tc_fence_after();
+            s_mma((g + 3) & 1, (g + 3) >> 1, ks.i, true);
+            ks.next();
+          }
+        }
+      }
+      g0 += w.nt;
     }
     // every MMA issued has completed before TMEM may be freed
     if (issuer) tc_commit(&bar.idle);
     __syncwarp();
-    (void)waitw(&bar.idle, 0, fail);
+    (void)waitw(fail, {&bar.idle, 0});
   } else if (warp >= SMX_WARPS && warp < MMA_WARP) {
     // ------------------------------------------------------------ conversion
     // A thread takes dims 16 c .. 16 c + 15 of every KSTEP-th key of a tile.  The 8
@@ -660,7 +716,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
           unsigned long long vis = ~0ull;
           if (key0 + TK > w.n) vis = visible(seen_by_any(a, w.b, lane), key0, w.n, w.kend) >> key;
           else vis >>= key;
-          if (!(ok = waitw(&bar.full[r.i], r.par, fail))) break;
+          if (!(ok = waitw(fail, {&bar.full[r.i], r.par}))) break;
           uint4 x[PER][2];
           uint32_t mx = 0;
 #pragma unroll
@@ -681,14 +737,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             mbar_arrive(&bar.dqmax[o]);
             mbar_arrive(&bar.empty[r.i]);
           }
-          if (!(ok = waitw(&bar.dqmax[o], g & 1, fail))) break;
+          if (!(ok = waitw(fail, {&bar.dqmax[o], uint32_t(g & 1)}))) break;
           float m = 0.f;
 #pragma unroll
           for (int i = 0; i < DQ_WARPS; ++i) m = fmaxf(m, s_dqmax[g & 1][o][i]);
           int e = top_exp(m, TOP16);
           if (o) {
             e = max(ev0, e);
-            ev0 = ev1;
+            ev0 = TWO ? e : ev1;
             ev1 = e;
           }
           if (d == 0) {
@@ -696,16 +752,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             else s_kmul[g & (EXPS - 1)] = pow2(e);
           }
           const float f = pow2(-e);
-          if (!(ok = waitw(&emptyb[q.i], q.par ^ 1, fail))) break;
+          if (!(ok = waitw(fail, {&emptyb[q.i], q.par ^ 1}))) break;
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
             *reinterpret_cast<uint4*>(dst + to[0] + i * (KSTEP * 128)) = conv16(x[i][0], f);
             *reinterpret_cast<uint4*>(dst + to[1] + i * (KSTEP * 128)) = conv16(x[i][1], f);
           }
         } else {
-          if (!(ok = waitw(&bar.prep[r.i], r.par, fail) && waitw(&bar.full[r.i], r.par, fail) &&
-                     waitw(&emptyb[q.i], q.par ^ 1, fail)))
-            break;
+          if (!(ok = waitw(fail, {&bar.prep[r.i], r.par}, {&bar.full[r.i], r.par}, {&emptyb[q.i], q.par ^ 1}))) break;
           const uint2* sc = reinterpret_cast<const uint2*>(sb + C::H_OFF + o * TK * G * 8) + key * G + (G == 2 ? c >> 2 : 0);
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
@@ -743,12 +797,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     int g0 = 0;
     bool ok = true;
     while (ok && w.next(a, nrb)) {
-      const int row0 = w.rb * ROWS, nrows = min(ROWS, R - row0);
+      const int row0 = (w.rb * C::BLOCKS + (TWO ? j : 0)) * ROWS, nrows = max(0, min(ROWS, R - row0));
       const int rep = repeats(nrows), per = ROWS / rep;
       const int lr = r % per, off = r / per * (TK / rep);  // row of the block, first of this lane's keys
       const bool row_ok = lr < nrows;
       const bool idle = lr - lane >= nrows;                // the whole warp has no row (per is a multiple of 32)
-      const int row = row0 + (row_ok ? lr : 0), qi = row / grp, h = w.hk * grp + row % grp;
+      const int row = row_ok ? row0 + lr : 0, qi = row / grp, h = w.hk * grp + row % grp;
       const unsigned long long word = a.anc[w.b * a.anc_sb + qi];
       // Q, scaled by a power of two per row; the sign of `scale` goes with it
       float c_row;
@@ -766,14 +820,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
         const float f = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
         c_row = fmaxf(fabsf(a.scale) * LOG2E * pow2(eq), 1e-37f);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {  // stream j stores half of the chunks
-          const int ch = j * (D / 16) + i;
-          const uint4 y = j ? x[D / 16 + i] : x[i];
-          uint4 o = conv16(y, f);
+        for (int i = 0; i < D / (TWO ? 8 : 16); ++i) {  // its block, or half of the chunks of the one block
+          const int ch = TWO ? i : j * (D / 16) + i;
+          uint4 o = conv16(!TWO && j ? x[(TWO ? 0 : D / 16) + i] : x[i], f);
           if constexpr (BITS == 4)  // positions 2 i + h hold dims i + 4 h, as the codes come
             o = make_uint4(__byte_perm(o.x, o.z, 0x5410), __byte_perm(o.x, o.z, 0x7632), __byte_perm(o.y, o.w, 0x5410),
                            __byte_perm(o.y, o.w, 0x7632));
-          *reinterpret_cast<uint4*>(qs + (ch >> 3) * (ROWS * 128) + sw128(r, ch & 7)) = o;
+          *reinterpret_cast<uint4*>(qs + (TWO ? j * C::QBLOCK : 0) + (ch >> 3) * (ROWS * 128) + sw128(r, ch & 7)) = o;
         }
         fence_async_smem();
         __syncwarp();
@@ -782,9 +835,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
       Row st{-INFINITY, 0.f, 0};
       int last = -1;  // this stream's last tile
 #pragma unroll 1
-      for (int g = g0 + ((g0 & 1) ^ j); g < g0 + w.nt && ok; g += 2) {
-        const int u = g >> 1, buf = 2 * j + (u & 1), key0 = (w.t0 + g - g0) * TK;
-        if (!(ok = waitw(&bar.sfull[buf], (u >> 1) & 1, fail))) break;
+      for (int g = TWO ? g0 : g0 + ((g0 & 1) ^ j); g < g0 + w.nt && ok; g += TWO ? 1 : 2) {
+        const int u = TWO ? g : g >> 1, buf = 2 * j + (u & 1), key0 = (w.t0 + g - g0) * TK;
+        if (!(ok = waitw(fail, {&bar.sfull[buf], uint32_t(u >> 1) & 1}))) break;
         if (!idle) {
           tc_fence_after();
           const bool edge = key0 + TK > w.n;
@@ -796,12 +849,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
                                   : softmax_tile<16>(st, sa, off, c, edge, vis);
           // V's exponent in this stream; for bf16 caches it is there once the tile's V is (whose
           // buffer cannot be refilled before this P is used: its phase stands still)
-          if (BITS == 0 && !(ok = waitw(&bar.vfull[g % NOP], (g / NOP) & 1, fail))) break;
+          if (BITS == 0 && !(ok = waitw(fail, {&bar.vfull[g % NOP], uint32_t(g / NOP) & 1}))) break;
           const int ev = s_ev[g & (EXPS - 1)];
           if (last >= 0) {
             if (ev != st.ev) corr *= pow2(max(st.ev - ev, -126));
             if (__any_sync(0xffffffffu, corr != 1.f)) {
-              if (!(ok = waitw(&bar.pvdone[j], (u - 1) & 1, fail))) break;
+              if (!(ok = waitw(fail, {&bar.pvdone[buf ^ 1], uint32_t((u - 1) >> 1) & 1}))) break;
               tc_fence_after();
               scale_o<D>(tmem + lrow + O_COL + 128u * j, corr);
             }
@@ -811,38 +864,39 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.pfull[j]);
+        if (lane == 0) mbar_arrive(&bar.pfull[buf]);
         last = u;
       }
       // ---- end of the run: both streams' O are complete
-      if (ok && last >= 0) ok = waitw(&bar.pvdone[j], last & 1, fail);
+      if (ok && last >= 0) ok = waitw(fail, {&bar.pvdone[2 * j + (last & 1)], uint32_t(last >> 1) & 1});
       s_row[j][r] = st;
       tc_fence_before();
       named_sync(1, SMX_WARPS * 32);
       tc_fence_after();
       if (tid == 0) s_stop = *fail;
       if (ok && !idle) {
-        const Row x = s_row[0][r], y = s_row[1][r];
+        // the two streams' states of the row, joined; TWO: the stream's own
+        const Row x = s_row[TWO ? j : 0][r], y = TWO ? Row{-INFINITY, 0.f, 0} : s_row[1][r];
         const float M = fmaxf(x.m, y.m);
         const float wx = x.m == -INFINITY ? 0.f : ex2(x.m - M), wy = y.m == -INFINITY ? 0.f : ex2(y.m - M);
         const float l = x.l * wx + y.l * wy;
         const bool direct = w.whole() && rep == 1;
         const float inv = direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
         const float fx = wx * pow2(x.ev) * inv, fy = wy * pow2(y.ev) * inv;
-        const size_t slot = size_t(cta_slot + w.pair) * ROWS + r;
+        const size_t slot = (size_t(blockIdx.x + w.pair) * C::BLOCKS + (TWO ? j : 0)) * ROWS + r;
         bf16* out = a.out + w.b * a.o_sb + h * a.o_sh + qi * a.o_sl;
 #pragma unroll 1
-        for (int i = 0; i < D / 2; i += 16) {  // stream j's warps write half of the dims
-          const int d0 = j * (D / 2) + i;
+        for (int i = 0; i < (TWO ? D : D / 2); i += 16) {  // TWO: all dims; else half of them
+          const int d0 = (TWO ? 0 : j * (D / 2)) + i;
           float o0[16], o1[16];
-          tmem_ld16(tmem + lrow + O_COL + d0, o0);
-          tmem_ld16(tmem + lrow + O_COL + 128u + d0, o1);
+          tmem_ld16(tmem + lrow + O_COL + (TWO ? 128u * j : 0u) + d0, o0);
+          if constexpr (!TWO) tmem_ld16(tmem + lrow + O_COL + 128u + d0, o1);
           tmem_ld_wait();
           float o[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             const int dim = BITS == 4 ? (k & 8) + ((k & 7) >> 1) + 4 * (k & 1) : k;
-            o[dim] = (wx > 0.f ? o0[k] * fx : 0.f) + (wy > 0.f ? o1[k] * fy : 0.f);
+            o[dim] = (wx > 0.f ? o0[k] * fx : 0.f) + (!TWO && wy > 0.f ? o1[k] * fy : 0.f);
           }
           if (!row_ok) continue;
           if (direct) {
@@ -861,7 +915,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             for (int k = 0; k < 4; ++k) po[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
         }
-        if (!direct && row_ok && j == 0) part_ml[slot] = make_float2(M, l);
+        if (!direct && row_ok && (TWO || j == 0)) part_ml[slot] = make_float2(M, l);
       }
       tc_fence_before();
       named_sync(1, SMX_WARPS * 32);  // O and Q may be overwritten
@@ -884,8 +938,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
 // The parts of a run are consecutive CTAs, each with `rep` repeats of the row.
 constexpr int JOIN_WARPS = 4;
 template <int D>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const TreeAttnArgs a, const int nrb, const int ctas,
-                                                                    const float* part_o, const float2* part_ml) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const TreeAttnArgs a, const int nrb, const int blocks,
+                                                                    const int ctas, const float* part_o,
+                                                                    const float2* part_ml) {
   constexpr int N = D / 32;
   __shared__ float s_m[JOIN_WARPS], s_l[JOIN_WARPS], s_o[JOIN_WARPS][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -900,18 +955,18 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const TreeAt
   }
   total = __reduce_add_sync(0xffffffffu, total);
   base = __reduce_add_sync(0xffffffffu, base);
-  const int tiles = seq_tiles(a, b), p = hk * nrb + rb, np = parts(total, ctas);
+  const int tiles = seq_tiles(a, b), p = hk * nrb + rb / blocks, np = parts(total, ctas);
   const int t0 = base + p * tiles, t1 = t0 + tiles - 1;
   // part c holds tile t: total * c / np <= t
   const int c0 = (int)(((t0 + 1LL) * np - 1) / total), c1 = (int)(((t1 + 1LL) * np - 1) / total);
   if (c0 == c1 && rep == 1) return;  // written by the attention kernel
   const int n = (c1 - c0 + 1) * rep;
-  const size_t slot0 = size_t(c0 + b * pairs + p) * ROWS + lr;
+  const size_t slot0 = (size_t(c0 + b * pairs + p) * blocks + rb % blocks) * ROWS + lr;
   float m = -INFINITY, l = 0.f, o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
   for (int i = warp; i < n; i += JOIN_WARPS) {
-    const size_t slot = slot0 + size_t(i / rep) * ROWS + (i % rep) * per;
+    const size_t slot = slot0 + size_t(i / rep) * blocks * ROWS + (i % rep) * per;
     const float2 ml = part_ml[slot];
     if (ml.x == -INFINITY) continue;
     const float mn = fmaxf(m, ml.x), c = m == -INFINITY ? 0.f : exp2f(m - mn), e = exp2f(ml.x - mn);
@@ -945,28 +1000,36 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const TreeAt
 }
 
 struct Plan {
-  int nrb, ctas;
+  int nrb, blocks, ctas;  // runs per kv head, row blocks of a run
   size_t slots;
 };
 static Plan plan(int B, int Hq, int Hkv, int L) {
-  const int nrb = ceil_div((long long)L * (Hq / Hkv), ROWS);
-  const int ctas = sm_count();
-  return {nrb, ctas, size_t(ctas) + size_t(B) * Hkv * nrb};
+  const long long rows = (long long)L * (Hq / Hkv);
+  const int blocks = rows > ROWS ? 2 : 1, nrb = ceil_div(rows, ROWS * blocks), ctas = sm_count();
+  return {nrb, blocks, ctas, (size_t(ctas) + size_t(B) * Hkv * nrb) * blocks};
 }
 
-template <int BITS, int D>
+template <int BITS, int D, bool TWO>
 static cudaError_t launch(const TreeAttnArgs& a, const Plan& p, cudaStream_t st) {
-  using C = Cfg<BITS, D>;
+  using C = Cfg<BITS, D, TWO>;
   static DeviceOnce once;
   cudaError_t e = once.run([&] {
-    return cudaFuncSetAttribute(tree_attn_kernel<BITS, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    return cudaFuncSetAttribute(tree_attn_kernel<BITS, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   });
   if (e != cudaSuccess) return e;
   float* po = reinterpret_cast<float*>(a.ws);
   float2* ml = reinterpret_cast<float2*>(po + p.slots * ROWS * D);
-  tree_attn_kernel<BITS, D><<<p.ctas, THREADS, C::SMEM, st>>>(a, p.nrb, po, ml);
-  tree_join_kernel<D><<<a.B * a.Hq * a.L, JOIN_WARPS * 32, 0, st>>>(a, p.nrb, p.ctas, po, ml);
+  tree_attn_kernel<BITS, D, TWO><<<p.ctas, THREADS, C::SMEM, st>>>(a, p.nrb, po, ml);
+  tree_join_kernel<D><<<a.B * a.Hq * a.L, JOIN_WARPS * 32, 0, st>>>(a, p.nrb, p.blocks, p.ctas, po, ml);
   return cudaGetLastError();
+}
+template <int BITS, int D>
+static cudaError_t launch(const TreeAttnArgs& a, const Plan& p, cudaStream_t st) {
+  return p.blocks == 2 ? launch<BITS, D, true>(a, p, st) : launch<BITS, D, false>(a, p, st);
+}
+template <int BITS>
+static cudaError_t launch(const TreeAttnArgs& a, const Plan& p, cudaStream_t st) {
+  return a.D == 64 ? launch<BITS, 64>(a, p, st) : launch<BITS, 128>(a, p, st);
 }
 
 }  // namespace atr
@@ -977,10 +1040,7 @@ size_t tree_attn_ws_bytes(int B, int Hq, int Hkv, int L, int D) {
 
 int tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st) {
   const atr::Plan p = atr::plan(a.B, a.Hq, a.Hkv, a.L);
-  cudaError_t e;
-  if (a.D == 64) e = a.bits == 8 ? atr::launch<8, 64>(a, p, st) : a.bits == 4 ? atr::launch<4, 64>(a, p, st) : atr::launch<0, 64>(a, p, st);
-  else e = a.bits == 8 ? atr::launch<8, 128>(a, p, st) : a.bits == 4 ? atr::launch<4, 128>(a, p, st) : atr::launch<0, 128>(a, p, st);
-  M5_CUDA(e);
+  M5_CUDA(a.bits == 8 ? atr::launch<8>(a, p, st) : a.bits == 4 ? atr::launch<4>(a, p, st) : atr::launch<0>(a, p, st));
   return M5_OK;
 }
 

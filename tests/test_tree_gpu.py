@@ -131,6 +131,35 @@ def test_attention(shape, D, bits):
 
 
 @pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("B,Hq,Hk,L,D,n", [(1, 16, 2, 2, 128, 70001), (1, 8, 2, 64, 128, 40000), (2, 4, 2, 24, 64, 60000),
+                                           (3, 24, 3, 40, 64, 9999)])
+def test_attention_long(bits, B, Hq, Hk, L, D, n):
+    """Dozens of tiles per CTA, so that every ring and buffer wraps many times and the warps of a CTA drift
+    apart: both against the definition and from call to call.  (rel is the bound of _check's 2-norm.)"""
+    from myinfer_b200 import _lib, ops
+    rng = np.random.default_rng(n + bits)
+    g = torch.Generator(device="cuda").manual_seed(n + bits)
+    rows, lengths = n + L + 1, [n - 17 * b for b in range(B)]
+    q = (1.5 * torch.randn(B, Hq, L, D, generator=g, device="cuda")).to(torch.bfloat16)
+    x, y = (torch.randn(B, Hk, rows, D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    k, v = ((ops.quantize(x, 64, bits), ops.quantize(y, 64, bits)) if bits else (x, y))
+    kd, vd = ((_dense(tuple(z.cpu() for z in t), bits) for t in (k, v)) if bits else (_f64(x), _f64(y)))
+    words = ref.ancestors(_trees(rng, B, L))[0]
+    out = _attend(q, k, v, lengths, words, D ** -0.5, L, bits)
+    for b in range(B):
+        hide = np.zeros((L, lengths[b] + L))
+        hide[:, lengths[b]:] = [[0.0 if int(words[b, i]) >> j & 1 else -math.inf for j in range(L)] for i in range(L)]
+        hide = torch.from_numpy(hide).cuda()
+        for h in range(Hq):
+            kh, vh = (torch.from_numpy(t[b, h // (Hq // Hk), :lengths[b] + L]).cuda() for t in (kd, vd))
+            want = torch.softmax(q[b, h].double() @ kh.T * D ** -0.5 + hide, 1) @ vh
+            assert ((out[b, h].double() - want).norm() / want.norm()).item() <= 5e-3
+    for _ in range(20):
+        assert torch.equal(out, _attend(q, k, v, lengths, words, D ** -0.5, L, bits))
+    _lib.device_check()
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
 def test_attention_masks_and_garbage(bits):
     """Rows that see nothing are zero; rows nobody sees may hold NaN and infinities."""
     rng = np.random.default_rng(5)
