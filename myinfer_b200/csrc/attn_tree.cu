@@ -12,29 +12,32 @@
 // inside a (sequence, head, row block) leaves a partial (max, sum, O) in the
 // workspace, joined by tree_join_kernel.
 //
-// Roles of a CTA (640 threads, registers moved to the softmax by setmaxnreg):
-//   warp 17      producer: bulk copies of 64-key tiles of K / V rows and of their
+// Roles of a CTA (896 threads, registers moved to the softmax by setmaxnreg):
+//   warp 25      producer: bulk copies of 64-key tiles of K / V rows and of their
 //                scales and biases (as the 16-byte blocks around them, so any
 //                2-byte alignment will do) into a ring;
-//   warps 18-19  scales, even and odd tiles: per tile and operand the exponent that puts the tile's largest value
+//   warps 26-27  scales, even and odd tiles: per tile and operand the exponent that puts the tile's largest value
 //                under 2^-2, and scale and bias in fp16 under it;
-//   warps 8-15   conversion to fp16, four warps for K and four for V, both into [key][dim] rows of
+//   warps 16-23  conversion to fp16, four warps for K and four for V, both into [key][dim] rows of
 //                128 bytes, 128-byte swizzle (K is read K-major, V MN-major: no transpose);
-//   warp 16      one thread issues the MMAs:  S = Q K^T  (Q, K in shared memory) and
+//   warp 24      one thread issues the MMAs:  S = Q K^T  (Q, K in shared memory) and
 //                O += P V  (P in tensor memory);
-//   warps 0-7    softmax.  Even and odd tiles are two independent streams of four
-//                warps each, with their own running maximum, sum and O, so that one's exponentials
-//                run beside the other's MMAs; S is double buffered within a
-//                stream and P overwrites the S it came from.
+//   warps 0-15   softmax.  Two independent streams of eight warps, each with its own running
+//                maximum, sum and O, so that one's exponentials run beside the other's
+//                MMAs: the even and the odd tiles of one block of 128 rows, or, above 128
+//                rows, the same tiles for two blocks.  Two warps share 32 rows of a
+//                stream and take half of a tile's keys each; they only exchange maxima when
+//                one of them moves (a barrier with an OR tells).  S is double buffered
+//                within a stream and P overwrites the S it came from.
 // Rounding: K, V and P are fp16 (2^-12 of the value or less; bf16 would cost as
 // much as the output's own rounding).  The exponents make that safe for
 // any range: an element's absolute error is at most 2^-23 of its tile's largest
 // value.  Q is scaled per row in the same way, which is exact.  Scores, maxima,
 // sums and O are fp32.  A row's maximum is only moved when a new score exceeds
 // it by 2^8 (p <= 256 in fp16): O is rescaled rarely.
-// With 64 rows or fewer, the idle rows repeat the rows and take a part of each
-// tile's keys (64 rows: halves, 32: quarters), which divides the exponentials
-// of a warp by 2 or 4; their states are joined like those of other CTAs.
+// With 64 rows or fewer, the idle lanes repeat the rows and take a part of each
+// tile's keys (64 rows: halves, 32: quarters), which divides the exponentials of a
+// warp by 2 or 4; their states are joined like those of other CTAs.
 // TMEM columns: S / P [stream][2] 64 each, O [stream] 128 each.
 #include <algorithm>
 #include <cmath>
@@ -50,12 +53,12 @@ namespace atr {
 
 constexpr int TK = 64;      // keys per tile
 constexpr int ROWS = 128;   // MMA M
-constexpr int SMX_WARPS = 8, DQ_WARPS = 4;  // conversion: DQ_WARPS for K and as many for V
+constexpr int SMX_WARPS = 16, DQ_WARPS = 4;  // conversion: DQ_WARPS for K and as many for V
 constexpr int MMA_WARP = SMX_WARPS + 2 * DQ_WARPS, PROD_WARP = MMA_WARP + 1, PREP_WARP = MMA_WARP + 2;
 constexpr int THREADS = (PREP_WARP + 2) * 32;
-// registers per thread after setmaxnreg: 2 + 2 + 1 warpgroups out of 640 x 96 at launch
-constexpr int SMX_REGS = 136, DQ_REGS = 72, MISC_REGS = 56;
-static_assert(256 * SMX_REGS + 256 * DQ_REGS + 128 * MISC_REGS <= 640 * 96, "register split");
+// registers per thread after setmaxnreg: 4 + 2 + 1 warpgroups out of 896 x 72 at launch
+constexpr int SMX_REGS = 80, DQ_REGS = 72, MISC_REGS = 40;
+static_assert(512 * SMX_REGS + 256 * DQ_REGS + 128 * MISC_REGS <= 896 * 72, "register split");
 constexpr int EXPS = 32;    // tile exponents held: more than the tiles between conversion and softmax
 constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -80,10 +83,11 @@ struct Cfg {
   static constexpr int STAGE = (H_OFF + (BITS ? 2 * TK * G * 8 : 0) + 127) / 128 * 128;
   static constexpr int OPER = TK * D * 2;                       // a converted tile
   static constexpr int NOP = TWO && BITS == 0 && D == 128 ? 2 : 3;  // converted K and V tiles held
+  static constexpr int CW = BITS ? DQ_WARPS / 2 : DQ_WARPS;     // conversion warps per tile and operand
   static constexpr int BLOCKS = TWO ? 2 : 1;
   static constexpr int QBLOCK = ROWS * D * 2, QBYTES = BLOCKS * QBLOCK;
   static constexpr int FIXED = QBYTES + 2 * NOP * OPER + 1024 + 1024;  // + alignment, barriers
-  static constexpr int ST = (227 * 1024 - 4096 - FIXED) / STAGE < 8 ? (227 * 1024 - 4096 - FIXED) / STAGE : 8;
+  static constexpr int ST = (227 * 1024 - 6656 - FIXED) / STAGE < 8 ? (227 * 1024 - 6656 - FIXED) / STAGE : 8;
   static constexpr int SMEM = FIXED + ST * STAGE;
 };
 
@@ -202,7 +206,7 @@ struct Slot {
 // block) runs of tiles(b) tiles.  32-bit counts: the host refuses longer lines.
 struct Line {
   int begin, end;  // this CTA's part
-  int b, base;     // sequence of tile `begin`, and that sequence's first tile
+  int b, base, n;  // sequence of tile `begin`, that sequence's first tile and committed keys
 };
 __device__ __forceinline__ int seq_len(const TreeAttnArgs& a, int b) {
   return ::min(::max(a.lengths[b], 0), (int)a.capacity);
@@ -213,29 +217,42 @@ __device__ __forceinline__ int seq_tiles(const TreeAttnArgs& a, int b) {
 }
 __device__ __forceinline__ int part_of(int total, int ctas, int c) { return (int)((long long)total * c / ctas); }
 __device__ __forceinline__ int parts(int total, int ctas) { return ::min(ctas, ::max(1, total / MIN_TILES)); }
-// by one warp: the tiles of all sequences; b_at and base_at: the sequence that
-// holds tile `at`, if any does
-__device__ __forceinline__ int scan_line(const TreeAttnArgs& a, int pairs, int lane, int at, int& b_at, int& base_at) {
-  int sum = 0;
-#pragma unroll 1
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
+// by one warp: this CTA's part of the line
+__device__ __forceinline__ Line part_of_line(const TreeAttnArgs& a, int pairs, int lane, int c, int ctas) {
+  Line l{0, 0, a.B - 1, 0, 0};
+  // pass 0 adds up all tiles, pass 1 finds the sequence (one chunk of 32 sequences: from the registers)
+  int total = 0, n = 0, w = 0, inc = 0;
+  auto chunk = [&](int b0) {
     const int b = b0 + lane;
-    const int w = b < a.B ? seq_tiles(a, b) * pairs : 0;
-    int inc = w;
+    n = b < a.B ? seq_len(a, b) : 0;
+    w = b < a.B ? (seq_end(a, n) + TK - 1) / TK * pairs : 0;
+    inc = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
-    const unsigned m = __ballot_sync(0xffffffffu, at >= sum + inc - w && at < sum + inc);
+    return __shfl_sync(0xffffffffu, inc, 31);
+  };
+#pragma unroll 1
+  for (int b0 = 0; b0 < a.B; b0 += 32) total += chunk(b0);
+  const int np = parts(total, ctas);
+  l.begin = c < np ? part_of(total, np, c) : total;
+  l.end = c < np ? part_of(total, np, c + 1) : total;
+#pragma unroll 1
+  for (int b0 = 0, sum = 0; b0 < a.B; b0 += 32) {
+    if (a.B > 32) chunk(b0);
+    const unsigned m = __ballot_sync(0xffffffffu, l.begin >= sum + inc - w && l.begin < sum + inc);
     if (m) {
       const int src = __ffs(m) - 1;
-      b_at = b0 + src;
-      base_at = sum + __shfl_sync(0xffffffffu, inc - w, src);
+      l.b = b0 + src;
+      l.base = sum + __shfl_sync(0xffffffffu, inc - w, src);
+      l.n = __shfl_sync(0xffffffffu, n, src);
+      break;
     }
     sum += __shfl_sync(0xffffffffu, inc, 31);
   }
-  return sum;
+  return l;
 }
 
 // Walks a CTA's part run by run; every role holds one and steps it alike.
@@ -244,16 +261,16 @@ struct Walk {
   int b, n, kend, tiles;        // sequence: committed keys, end of its keys, tiles
   int hk, rb, t0, nt, pair;     // run: kv head, row block, first tile, tiles of this part; pair = its number
   __device__ __forceinline__ Walk(const Line& l, const TreeAttnArgs& a)
-      : at(l.begin), end(l.end), base(l.base), b(l.b), tiles(0) {}
+      : at(l.begin), end(l.end), base(l.base), b(l.b), n(l.n) {
+    kend = seq_end(a, n);
+    tiles = (kend + TK - 1) / TK;
+  }
   __device__ __forceinline__ bool next(const TreeAttnArgs& a, int nrb) {
     if (at >= end) return false;
     const int pairs = a.Hkv * nrb;
-    if (tiles && at - base >= tiles * pairs) {
+    if (at - base >= tiles * pairs) {
       base += tiles * pairs;
       ++b;
-      tiles = 0;
-    }
-    if (!tiles) {
       n = seq_len(a, b);
       kend = seq_end(a, n);
       tiles = (kend + TK - 1) / TK;
@@ -310,55 +327,59 @@ __device__ __forceinline__ uint4 conv16(uint4 w, float f) {
                     h2(bf16_lo(w.z) * f, bf16_hi(w.z) * f), h2(bf16_lo(w.w) * f, bf16_hi(w.w) * f));
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
-// State of one row in one stream.
-struct Row {
-  float m, l;  // maximum in log2 units (-inf: nothing seen), sum of p
-  int ev;      // O holds its sum divided by 2^ev
-};
-
-// O *= f for this thread's row.
+// O *= f over D dims of this thread's row.
 template <int D>
 __device__ __forceinline__ void scale_o(uint32_t o_addr, float f) {
 #pragma unroll 1
-  for (int d = 0; d < D; d += 32) {
-    float o[32];
-    tmem_ld32(o_addr + d, o);
+  for (int d = 0; d < D; d += 16) {
+    float o[16];
+    tmem_ld16(o_addr + d, o);
     tmem_ld_wait();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) o[i] *= f;
-    tmem_st32(o_addr + d, reinterpret_cast<const uint32_t*>(o));
+    for (int i = 0; i < 16; ++i) o[i] *= f;
+    tmem_st16(o_addr + d, reinterpret_cast<const uint32_t(&)[16]>(o));
   }
 }
 
-// One tile of a softmax thread: N of the tile's 64 keys, from `off` on; P of the
-// other keys is zero.  Returns the factor by which O has to change.
+// Meets the other warp of a row quarter; whether `p` holds for any of the 64 lanes.
+__device__ __forceinline__ bool pair_or(int id, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(id), "r"(uint32_t(p))
+      : "memory");
+  return r != 0;
+}
+
+// State of one row in one stream, kept by both warps that share it.
+struct Row {
+  float m, l;  // maximum in log2 units (-inf: nothing seen); this warp's part of the sum of p
+  int ev;      // O holds its sum divided by 2^ev
+};
+
+// One tile of a softmax thread: N of the tile's 64 keys, from `off` on, into the P
+// columns of those keys.  pair: barrier of the two warps that share the
+// rows (0: this warp has them alone), mine / other: where they exchange maxima.
+// Returns the factor by which O has to change.
 template <int N>
 __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, float c, bool edge,
-                                              unsigned long long vis) {
+                                              unsigned long long vis, int pair, float* mine, const float* other) {
   float s[N];
-  if constexpr (N == 16) {
-    tmem_ld16(s_addr + off, s);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 32) tmem_ld32(s_addr + off + i, *reinterpret_cast<float(*)[32]>(s + i));
-  }
+  if constexpr (N == 32) tmem_ld32(s_addr + off, s);
+  else tmem_ld16(s_addr + off, s);
   tmem_ld_wait();
   if (edge) {
-    const uint32_t v[2] = {uint32_t(vis >> off), uint32_t((vis >> off) >> 32)};
+    const uint32_t v = uint32_t(vis >> off);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (!((v[i / 32] >> (i % 32)) & 1)) s[i] = -INFINITY;
+      if (!((v >> i) & 1)) s[i] = -INFINITY;
   }
   float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -367,12 +388,20 @@ __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, 
     for (int j = 0; j < 4; ++j) mx[j] = i + 4 + j < N ? max3(mx[j], s[i + j], s[i + 4 + j]) : fmaxf(mx[j], s[i + j]);
   }
   const float tmax = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
-  const float mt = tmax == -INFINITY ? -INFINITY : tmax * c;
-  float corr = 1.f;
-  if (mt > r.m + LAZY) {  // also: the first score the row sees (r.m = -inf)
-    corr = r.m == -INFINITY ? 0.f : ex2(r.m - mt);
-    r.m = mt;
-    r.l *= corr;
+  float mt = tmax == -INFINITY ? -INFINITY : tmax * c, corr = 1.f;
+  const bool up = mt > r.m + LAZY;  // also: the first score the row sees (r.m = -inf)
+  // both warps have read their S here, so either's P may overwrite it
+  if (pair ? pair_or(pair, up) : __any_sync(0xffffffffu, up)) {
+    if (pair) {
+      *mine = mt;
+      named_sync(pair, 64);
+      mt = fmaxf(mt, *other);
+    }
+    if (mt > r.m + LAZY) {
+      corr = r.m == -INFINITY ? 0.f : ex2(r.m - mt);
+      r.m = mt;
+      r.l *= corr;
+    }
   }
   const float neg = r.m == -INFINITY ? 0.f : -r.m;
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -385,25 +414,13 @@ __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, 
     p[i / 2] = h2(e.x, e.y);
   }
   r.l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-  if constexpr (N == 64) {
-    tmem_st32(s_addr, p);
-  } else {
-    uint32_t z[16];
-#pragma unroll
-    for (int k = 0; k < 64; k += 32) {  // 32 keys = 16 columns at a time
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if constexpr (N == 32) z[i] = k == off ? p[i] : 0u;
-        else z[i] = k + (i >= 8 ? 16 : 0) == off ? p[i & 7] : 0u;
-      }
-      tmem_st16(s_addr + k / 2, z);
-    }
-  }
+  if constexpr (N == 32) tmem_st16(s_addr + off / 2, p);
+  else tmem_st8(s_addr + off / 2, p);
   return corr;
 }
 
 template <int BITS, int D, bool TWO>
-__global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArgs a, const int nrb, float* part_o,
+__global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArgs a, const int nrb, float4* part_o,
                                                                float2* part_ml) {
   using C = Cfg<BITS, D, TWO>;
   constexpr int ST = C::ST, G = C::G, NOP = C::NOP;
@@ -415,7 +432,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
   uint8_t* ring = vop + NOP * C::OPER;
   Bars<ST, NOP>& bar = *reinterpret_cast<Bars<ST, NOP>*>(ring + ST * C::STAGE);
   static_assert(sizeof(Bars<ST, NOP>) <= 1024, "barriers");
-  __shared__ Row s_row[2][ROWS];
+  __shared__ float s_m[2][ROWS], s_xl[2][2][ROWS];  // at a run's end; s_xl [stream][half] also: maxima exchanged
+  __shared__ int s_oev[2][ROWS];
+  __shared__ uint32_t s_qmax[4][ROWS];
   __shared__ float s_kmul[EXPS];
   __shared__ int s_ev[EXPS];
   __shared__ float s_dqmax[2][2][DQ_WARPS];  // [tile parity][K, V]
@@ -431,12 +450,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     s_fail = 0;
     for (int i = 0; i < ST; ++i) {
       mbar_init(&bar.full[i], 1);
-      mbar_init(&bar.empty[i], 2 * DQ_WARPS);
+      mbar_init(&bar.empty[i], 2 * C::CW);
       mbar_init(&bar.prep[i], 1);
     }
     for (int i = 0; i < NOP; ++i) {
-      mbar_init(&bar.kfull[i], DQ_WARPS);
-      mbar_init(&bar.vfull[i], DQ_WARPS);
+      mbar_init(&bar.kfull[i], C::CW);
+      mbar_init(&bar.vfull[i], C::CW);
       mbar_init(&bar.kempty[i], 1);
       mbar_init(&bar.vempty[i], 1);
     }
@@ -454,13 +473,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     tmem_alloc(&s_tmem, TMEM_COLS);
     tmem_relinquish();
   }
+  pdl_launch_dependents();
+  pdl_wait();
   if (warp == 0) {
-    Line l{0, 0, a.B - 1, 0};
-    const int total = scan_line(a, a.Hkv * nrb, lane, -1, l.b, l.base);
-    const int np = parts(total, gridDim.x), c = blockIdx.x;
-    l.begin = c < np ? part_of(total, np, c) : total;
-    l.end = c < np ? part_of(total, np, c + 1) : total;
-    scan_line(a, a.Hkv * nrb, lane, l.begin, l.b, l.base);
+    const Line l = part_of_line(a, a.Hkv * nrb, lane, blockIdx.x, gridDim.x);
     if (lane == 0) s_line = l;
   }
   tc_fence_before();
@@ -683,8 +699,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     // one key with the halves of 4-7 in the other order (bf16 rows of 256 bytes).
     setmaxnreg_dec<DQ_REGS>();
     const int o = warp >= SMX_WARPS + DQ_WARPS;  // K, V
-    const int d = tid - (SMX_WARPS + o * DQ_WARPS) * 32;
-    constexpr int PIECES = D / 16, KSTEP = DQ_WARPS * 32 / PIECES, PER = TK / KSTEP;
+    // Packed caches: two warps convert the even tiles of an operand and two the odd ones (a tile's
+    // chain of waits, loads, stores and fence is latency, which two tiles at once hide).
+    // bf16 caches: all four every tile (they take its maximum first, and V's runs on).
+    const int turn = (warp - SMX_WARPS) % DQ_WARPS / C::CW;
+    const int d = (tid - SMX_WARPS * 32) % (C::CW * 32);
+    constexpr int PIECES = D / 16, KSTEP = C::CW * 32 / PIECES, PER = TK / KSTEP;
     const int c = d % PIECES;
     const int key = G == 2 && BITS != 0 ? 2 * (d >> 4) + (((d >> 2) ^ (d >> 3)) & 1) : d / PIECES;
     const int swap = G == 2 && BITS == 0 ? c >> 2 : 0;  // order of the two 8-dim chunks
@@ -707,7 +727,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     while (ok && w.next(a, nrb)) {
       int ev0 = -127, ev1 = -127;
 #pragma unroll 1
-      for (int t = 0; t < w.nt; ++t, ++g) {
+      for (int t = 0; t < w.nt; ++t, ++g, r.next(), q.next()) {
+        if (BITS != 0 && (g & 1) != turn) continue;
         const uint8_t* sb = ring + r.i * C::STAGE;
         const uint8_t* src = sb + from0;
         uint8_t* dst = oper + q.i * C::OPER;
@@ -784,45 +805,55 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
           mbar_arrive(&fullb[q.i]);
           if (BITS != 0) mbar_arrive(&bar.empty[r.i]);
         }
-        r.next();
-        q.next();
       }
     }
   } else if (warp < SMX_WARPS) {
     // ---------------------------------------------------------------- softmax
     setmaxnreg_inc<SMX_REGS>();
-    const int j = warp >> 2, r = tid & 127;      // stream, lane of tensor memory
+    const int j = warp >> 3, h = (warp >> 2) & 1, r = tid & 127;  // stream, half of the keys, lane of tensor memory
     const uint32_t lrow = uint32_t(32 * (warp & 3)) << 16;
+    constexpr int QPARTS = TWO ? 2 : 4;           // warps that share a row: of its stream, of both
+    const int qp = TWO ? h : 2 * j + h;
+    const int pair_id = 2 + 4 * j + (warp & 3);   // barriers 2-9
     Walk w(line, a);
     int g0 = 0;
     bool ok = true;
     while (ok && w.next(a, nrb)) {
       const int row0 = (w.rb * C::BLOCKS + (TWO ? j : 0)) * ROWS, nrows = max(0, min(ROWS, R - row0));
       const int rep = repeats(nrows), per = ROWS / rep;
-      const int lr = r % per, off = r / per * (TK / rep);  // row of the block, first of this lane's keys
+      const int lr = r % per, rr = r / per;         // row of the block, its repeat
       const bool row_ok = lr < nrows;
-      const bool idle = lr - lane >= nrows;                // the whole warp has no row (per is a multiple of 32)
-      const int row = row_ok ? row0 + lr : 0, qi = row / grp, h = w.hk * grp + row % grp;
+      const int row = row_ok ? row0 + lr : 0, qi = row / grp, hq = w.hk * grp + row % grp;
+      // keys of this warp: 32 h (one repeat), 32 rr + 16 h (two), 16 rr (four: half 0 alone)
+      const int off = rep == 1 ? 32 * h : rep == 2 ? 32 * rr + 16 * h : 16 * rr;
+      const bool idle = lr - lane >= nrows || (rep == 4 && h);  // nothing to do for the whole warp (per is a multiple of 32)
+      const int pair = rep == 4 || lr - lane >= nrows ? 0 : pair_id;
       const unsigned long long word = a.anc[w.b * a.anc_sb + qi];
       // Q, scaled by a power of two per row; the sign of `scale` goes with it
       float c_row;
       {
-        const uint4* qr = reinterpret_cast<const uint4*>(a.q + w.b * a.q_sb + h * a.q_sh + qi * a.q_sl);
-        uint4 x[D / 8];
+        constexpr int NQ = D / 8 / QPARTS;  // chunks of 8 dims per warp
+        const uint4* qr = reinterpret_cast<const uint4*>(a.q + w.b * a.q_sb + hq * a.q_sh + qi * a.q_sl) + qp * NQ;
+        uint4 x[NQ];
         uint32_t mx = 0;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) x[i] = row_ok ? qr[i] : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < NQ; ++i) x[i] = row_ok ? qr[i] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
+        for (int i = 0; i < NQ; ++i)
           mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu),
                                      __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
+        // the largest exponent of the whole row
+        s_qmax[2 * j + h][r] = mx;
+        named_sync(1, SMX_WARPS * 32);
+#pragma unroll
+        for (int i = 0; i < QPARTS; ++i) mx = __vmaxu2(mx, s_qmax[TWO ? 2 * j + i : i][r]);
         const int eq = top_exp(__uint_as_float(max(mx & 0xFFFFu, mx >> 16) << 16), TOP16);
         const float f = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
         c_row = fmaxf(fabsf(a.scale) * LOG2E * pow2(eq), 1e-37f);
 #pragma unroll
-        for (int i = 0; i < D / (TWO ? 8 : 16); ++i) {  // its block, or half of the chunks of the one block
-          const int ch = TWO ? i : j * (D / 16) + i;
-          uint4 o = conv16(!TWO && j ? x[(TWO ? 0 : D / 16) + i] : x[i], f);
+        for (int i = 0; i < NQ; ++i) {
+          const int ch = qp * NQ + i;
+          uint4 o = conv16(x[i], f);
           if constexpr (BITS == 4)  // positions 2 i + h hold dims i + 4 h, as the codes come
             o = make_uint4(__byte_perm(o.x, o.z, 0x5410), __byte_perm(o.x, o.z, 0x7632), __byte_perm(o.y, o.w, 0x5410),
                            __byte_perm(o.y, o.w, 0x7632));
@@ -834,29 +865,43 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
       }
       Row st{-INFINITY, 0.f, 0};
       int last = -1;  // this stream's last tile
+      // After a wait that ran out the loop goes on without waiting: the warps of a pair meet in every tile.
 #pragma unroll 1
-      for (int g = TWO ? g0 : g0 + ((g0 & 1) ^ j); g < g0 + w.nt && ok; g += TWO ? 1 : 2) {
+      for (int g = TWO ? g0 : g0 + ((g0 & 1) ^ j); g < g0 + w.nt; g += TWO ? 1 : 2) {
         const int u = TWO ? g : g >> 1, buf = 2 * j + (u & 1), key0 = (w.t0 + g - g0) * TK;
-        if (!(ok = waitw(fail, {&bar.sfull[buf], uint32_t(u >> 1) & 1}))) break;
+        ok = ok && waitw(fail, {&bar.sfull[buf], uint32_t(u >> 1) & 1});
         if (!idle) {
           tc_fence_after();
           const bool edge = key0 + TK > w.n;
           const unsigned long long vis = edge ? visible(word, key0, w.n, w.kend) : 0ull;
           const float c = c_row * s_kmul[g & (EXPS - 1)];
           const uint32_t sa = tmem + lrow + S_COL + 64u * buf;
-          float corr = rep == 1   ? softmax_tile<64>(st, sa, 0, c, edge, vis)
-                       : rep == 2 ? softmax_tile<32>(st, sa, off, c, edge, vis)
-                                  : softmax_tile<16>(st, sa, off, c, edge, vis);
+          float corr;
+          if (rep == 1) {
+            corr = softmax_tile<32>(st, sa, off, c, edge, vis, pair, &s_xl[j][h][r], &s_xl[j][h ^ 1][r]);
+          } else {
+            corr = softmax_tile<16>(st, sa, off, c, edge, vis, pair, &s_xl[j][h][r], &s_xl[j][h ^ 1][r]);
+            // P of the keys other repeats take is zero: half of them, or (one warp) all
+            const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+            if (rep == 2) {
+              tmem_st8(sa + 16u * (rr ^ 1) + 8u * h, z);
+            } else {
+#pragma unroll
+              for (int k = 1; k < 4; ++k) tmem_st8(sa + 8u * ((rr + k) & 3), z);
+            }
+          }
           // V's exponent in this stream; for bf16 caches it is there once the tile's V is (whose
           // buffer cannot be refilled before this P is used: its phase stands still)
-          if (BITS == 0 && !(ok = waitw(fail, {&bar.vfull[g % NOP], uint32_t(g / NOP) & 1}))) break;
+          if (BITS == 0) ok = ok && waitw(fail, {&bar.vfull[g % NOP], uint32_t(g / NOP) & 1});
           const int ev = s_ev[g & (EXPS - 1)];
           if (last >= 0) {
             if (ev != st.ev) corr *= pow2(max(st.ev - ev, -126));
-            if (__any_sync(0xffffffffu, corr != 1.f)) {
-              if (!(ok = waitw(fail, {&bar.pvdone[buf ^ 1], uint32_t((u - 1) >> 1) & 1}))) break;
+            if (__any_sync(0xffffffffu, corr != 1.f)) {  // the same for both warps: each takes half of the dims
+              ok = ok && waitw(fail, {&bar.pvdone[buf ^ 1], uint32_t((u - 1) >> 1) & 1});
               tc_fence_after();
-              scale_o<D>(tmem + lrow + O_COL + 128u * j, corr);
+              const uint32_t oa = tmem + lrow + O_COL + 128u * j;
+              if (pair) scale_o<D / 2>(oa + h * (D / 2), corr);
+              else scale_o<D>(oa, corr);
             }
           }
           st.ev = ev;
@@ -869,27 +914,31 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
       }
       // ---- end of the run: both streams' O are complete
       if (ok && last >= 0) ok = waitw(fail, {&bar.pvdone[2 * j + (last & 1)], uint32_t(last >> 1) & 1});
-      s_row[j][r] = st;
+      s_xl[j][h][r] = idle ? 0.f : st.l;
+      if (h == 0) {
+        s_m[j][r] = st.m;
+        s_oev[j][r] = st.ev;
+      }
       tc_fence_before();
       named_sync(1, SMX_WARPS * 32);
       tc_fence_after();
       if (tid == 0) s_stop = *fail;
-      if (ok && !idle) {
+      if (ok && lr - lane < nrows) {
         // the two streams' states of the row, joined; TWO: the stream's own
-        const Row x = s_row[TWO ? j : 0][r], y = TWO ? Row{-INFINITY, 0.f, 0} : s_row[1][r];
-        const float M = fmaxf(x.m, y.m);
-        const float wx = x.m == -INFINITY ? 0.f : ex2(x.m - M), wy = y.m == -INFINITY ? 0.f : ex2(y.m - M);
-        const float l = x.l * wx + y.l * wy;
+        const int j0 = TWO ? j : 0;
+        const float mx = s_m[j0][r], my = TWO ? -INFINITY : s_m[1][r], M = fmaxf(mx, my);
+        const float wx = mx == -INFINITY ? 0.f : ex2(mx - M), wy = my == -INFINITY ? 0.f : ex2(my - M);
+        float l = (s_xl[j0][0][r] + s_xl[j0][1][r]) * wx;
+        if constexpr (!TWO) l += (s_xl[1][0][r] + s_xl[1][1][r]) * wy;
         const bool direct = w.whole() && rep == 1;
         const float inv = direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
-        const float fx = wx * pow2(x.ev) * inv, fy = wy * pow2(y.ev) * inv;
-        const size_t slot = (size_t(blockIdx.x + w.pair) * C::BLOCKS + (TWO ? j : 0)) * ROWS + r;
-        bf16* out = a.out + w.b * a.o_sb + h * a.o_sh + qi * a.o_sl;
+        const float fx = wx * pow2(s_oev[j0][r]) * inv, fy = TWO ? 0.f : wy * pow2(s_oev[1][r]) * inv;
+        const size_t slot = size_t(blockIdx.x + w.pair) * C::BLOCKS + (TWO ? j : 0);
+        bf16* out = a.out + w.b * a.o_sb + hq * a.o_sh + qi * a.o_sl;
 #pragma unroll 1
-        for (int i = 0; i < (TWO ? D : D / 2); i += 16) {  // TWO: all dims; else half of them
-          const int d0 = (TWO ? 0 : j * (D / 2)) + i;
+        for (int d0 = qp * (D / QPARTS); d0 < (qp + 1) * (D / QPARTS); d0 += 16) {
           float o0[16], o1[16];
-          tmem_ld16(tmem + lrow + O_COL + (TWO ? 128u * j : 0u) + d0, o0);
+          tmem_ld16(tmem + lrow + O_COL + 128u * j0 + d0, o0);
           if constexpr (!TWO) tmem_ld16(tmem + lrow + O_COL + 128u + d0, o1);
           tmem_ld_wait();
           float o[16];
@@ -910,17 +959,17 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             reinterpret_cast<uint4*>(out + d0)[0] = v[0];
             reinterpret_cast<uint4*>(out + d0)[1] = v[1];
           } else {
-            float4* po = reinterpret_cast<float4*>(part_o + slot * D + d0);
+            float4* po = part_o + (slot * (D / 4) + d0 / 4) * ROWS + r;  // [slot][dim / 4][row]: rows side by side
 #pragma unroll
-            for (int k = 0; k < 4; ++k) po[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            for (int k = 0; k < 4; ++k) po[k * ROWS] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
         }
-        if (!direct && row_ok && (TWO || j == 0)) part_ml[slot] = make_float2(M, l);
+        if (!direct && row_ok && qp == 0) part_ml[slot * ROWS + r] = make_float2(M, l);
       }
       tc_fence_before();
       named_sync(1, SMX_WARPS * 32);  // O and Q may be overwritten
       tc_fence_after();
-      ok = !s_stop;  // one answer for the eight warps: they meet at the barriers of the next run or leave together
+      ok = !s_stop;  // one answer for all warps: they meet at the barriers of the next run or leave together
       g0 += w.nt;
     }
   }
@@ -933,20 +982,27 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
   }
 }
 
-// Joins the partial states of the rows whose run was cut: one CTA per (row block of a
-// kv head, row): o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max).
-// The parts of a run are consecutive CTAs, each with `rep` repeats of the row.
-constexpr int JOIN_WARPS = 4;
-template <int D>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const TreeAttnArgs a, const int nrb, const int blocks,
-                                                                    const int ctas, const float* part_o,
-                                                                    const float2* part_ml) {
-  constexpr int N = D / 32;
-  __shared__ float s_m[JOIN_WARPS], s_l[JOIN_WARPS], s_o[JOIN_WARPS][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Joins the partial states of the rows whose run was cut or that were repeated:
+//   o = sum_i w_i O_i / sum_i w_i l_i,  w_i = 2^(m_i - max).
+// One CTA per block of 128 lanes and 16 dims; a thread takes one lane of
+// every second part (the parts of a run are consecutive CTAs), so all loads run
+// along the lanes.  The repeats of a row and the two halves meet in shared memory.
+constexpr int JOIN_DIMS = 16;
+__global__ void __launch_bounds__(2 * ROWS) tree_join_kernel(const TreeAttnArgs a, const int nrb, const int blocks,
+                                                             const int ctas, const float4* part_o,
+                                                             const float2* part_ml) {
+  __shared__ float s_m[2][ROWS], s_l[2][ROWS], s_o[2][ROWS][JOIN_DIMS + 1];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, r = tid & (ROWS - 1), half = tid / ROWS;
   const int grp = a.Hq / a.Hkv, R = a.L * grp, pairs = a.Hkv * nrb;
-  const int row = blockIdx.x % R, hk = blockIdx.x / R % a.Hkv, b = blockIdx.x / R / a.Hkv;
-  const int rb = row / ROWS, lr = row % ROWS, rep = repeats(min(ROWS, R - rb * ROWS)), per = ROWS / rep;
+  int x = blockIdx.x;
+  const int blk = x % blocks;
+  x /= blocks;
+  const int p = x % pairs, b = x / pairs;
+  const int row0 = (p % nrb * blocks + blk) * ROWS, nrows = min(ROWS, R - row0);
+  if (nrows <= 0) return;
+  const int rep = repeats(nrows), per = ROWS / rep;
   int total = 0, base = 0;  // tiles of all sequences, and of those before b
   for (int i = lane; i < a.B; i += 32) {
     const int t = seq_tiles(a, i) * pairs;
@@ -955,48 +1011,89 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const TreeAt
   }
   total = __reduce_add_sync(0xffffffffu, total);
   base = __reduce_add_sync(0xffffffffu, base);
-  const int tiles = seq_tiles(a, b), p = hk * nrb + rb / blocks, np = parts(total, ctas);
+  const int tiles = seq_tiles(a, b), np = parts(total, ctas);
   const int t0 = base + p * tiles, t1 = t0 + tiles - 1;
   // part c holds tile t: total * c / np <= t
   const int c0 = (int)(((t0 + 1LL) * np - 1) / total), c1 = (int)(((t1 + 1LL) * np - 1) / total);
   if (c0 == c1 && rep == 1) return;  // written by the attention kernel
-  const int n = (c1 - c0 + 1) * rep;
-  const size_t slot0 = (size_t(c0 + b * pairs + p) * blocks + rb % blocks) * ROWS + lr;
-  float m = -INFINITY, l = 0.f, o[N];
+  const int n = c1 - c0 + 1, d4 = blockIdx.y * (JOIN_DIMS / 4), D4 = a.D / 4;
+  const size_t slot0 = size_t(c0 + b * pairs + p) * blocks + blk;
+  const bool mine = r % per < nrows;
+  const float2* ml = part_ml + slot0 * ROWS + r;
+  const float4* po = part_o + (slot0 * D4 + d4) * ROWS + r;
+  float m = -INFINITY, l = 0.f;
+  float4 o[JOIN_DIMS / 4];
 #pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = 0.f;
-  for (int i = warp; i < n; i += JOIN_WARPS) {
-    const size_t slot = slot0 + size_t(i / rep) * blocks * ROWS + (i % rep) * per;
-    const float2 ml = part_ml[slot];
-    if (ml.x == -INFINITY) continue;
-    const float mn = fmaxf(m, ml.x), c = m == -INFINITY ? 0.f : exp2f(m - mn), e = exp2f(ml.x - mn);
-    m = mn;
-    l = l * c + ml.y * e;
-    const float* po = part_o + slot * D + lane * N;
+  for (int k = 0; k < JOIN_DIMS / 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (mine) {
+#pragma unroll 4
+    for (int i = half; i < n; i += 2) m = fmaxf(m, ml[size_t(i) * blocks * ROWS].x);
+#pragma unroll 2
+    for (int i = half; i < n; i += 2) {
+      const float2 e = ml[size_t(i) * blocks * ROWS];
+      const float w = e.x == -INFINITY ? 0.f : ex2(e.x - m);
+      l = fmaf(w, e.y, l);
 #pragma unroll
-    for (int k = 0; k < N; ++k) o[k] = fmaf(po[k], e, o[k] * c);
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) s_o[warp][lane * N + i] = o[i];
-  __syncthreads();
-  float M = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < JOIN_WARPS; ++i) M = fmaxf(M, s_m[i]);
-  const int qi = row / grp, h = hk * grp + row % grp;
-  for (int d = threadIdx.x; d < D; d += JOIN_WARPS * 32) {
-    float num = 0.f, den = 0.f;
-#pragma unroll
-    for (int i = 0; i < JOIN_WARPS; ++i) {
-      const float c = s_m[i] == -INFINITY ? 0.f : exp2f(s_m[i] - M);
-      num = fmaf(c, s_o[i][d], num);
-      den = fmaf(c, s_l[i], den);
+      for (int k = 0; k < JOIN_DIMS / 4; ++k) {
+        const float4 v = po[(size_t(i) * blocks * D4 + k) * ROWS];
+        o[k].x = fmaf(w, v.x, o[k].x);
+        o[k].y = fmaf(w, v.y, o[k].y);
+        o[k].z = fmaf(w, v.z, o[k].z);
+        o[k].w = fmaf(w, v.w, o[k].w);
+      }
     }
-    a.out[b * a.o_sb + h * a.o_sh + qi * a.o_sl + d] = f2bf(den == 0.f ? 0.f : num / den);
   }
+  s_m[half][r] = m;
+  s_l[half][r] = l;
+#pragma unroll
+  for (int k = 0; k < JOIN_DIMS / 4; ++k) {
+    s_o[half][r][4 * k] = o[k].x;
+    s_o[half][r][4 * k + 1] = o[k].y;
+    s_o[half][r][4 * k + 2] = o[k].z;
+    s_o[half][r][4 * k + 3] = o[k].w;
+  }
+  __syncthreads();
+  // two threads per row, 8 dims each
+  const int lr = tid >> 1, dh = (tid & 1) * (JOIN_DIMS / 2);
+  if (lr >= nrows) return;
+  float M = -INFINITY;
+  for (int i = 0; i < 2 * rep; ++i) M = fmaxf(M, s_m[i & 1][lr + (i >> 1) * per]);
+  float den = 0.f, num[JOIN_DIMS / 2];
+#pragma unroll
+  for (int k = 0; k < JOIN_DIMS / 2; ++k) num[k] = 0.f;
+  for (int i = 0; i < 2 * rep; ++i) {
+    const int q = lr + (i >> 1) * per;
+    const float w = s_m[i & 1][q] == -INFINITY ? 0.f : ex2(s_m[i & 1][q] - M);
+    den = fmaf(w, s_l[i & 1][q], den);
+#pragma unroll
+    for (int k = 0; k < JOIN_DIMS / 2; ++k) num[k] = fmaf(w, s_o[i & 1][q][dh + k], num[k]);
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const int row = row0 + lr, qi = row / grp, h = p / nrb * grp + row % grp;
+  uint32_t v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __nv_bfloat162 z = __floats2bfloat162_rn(num[2 * k] * inv, num[2 * k + 1] * inv);
+    v[k] = *reinterpret_cast<const uint32_t*>(&z);
+  }
+  *reinterpret_cast<uint4*>(a.out + b * a.o_sb + h * a.o_sh + qi * a.o_sl + 4 * d4 + dh) = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// Launch that may begin while the kernel before it on the stream ends (both
+// kernels wait for it before they read or write anything in global memory).
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_early(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 
 struct Plan {
@@ -1017,11 +1114,12 @@ static cudaError_t launch(const TreeAttnArgs& a, const Plan& p, cudaStream_t st)
     return cudaFuncSetAttribute(tree_attn_kernel<BITS, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   });
   if (e != cudaSuccess) return e;
-  float* po = reinterpret_cast<float*>(a.ws);
-  float2* ml = reinterpret_cast<float2*>(po + p.slots * ROWS * D);
-  tree_attn_kernel<BITS, D, TWO><<<p.ctas, THREADS, C::SMEM, st>>>(a, p.nrb, po, ml);
-  tree_join_kernel<D><<<a.B * a.Hq * a.L, JOIN_WARPS * 32, 0, st>>>(a, p.nrb, p.blocks, p.ctas, po, ml);
-  return cudaGetLastError();
+  float4* po = reinterpret_cast<float4*>(a.ws);
+  float2* ml = reinterpret_cast<float2*>(po + p.slots * ROWS * (D / 4));
+  if ((e = launch_early(tree_attn_kernel<BITS, D, TWO>, dim3(p.ctas), dim3(THREADS), C::SMEM, st, a, p.nrb, po, ml)))
+    return e;
+  return launch_early(tree_join_kernel, dim3(a.B * a.Hkv * p.nrb * p.blocks, D / JOIN_DIMS), dim3(2 * ROWS), 0, st, a,
+                      p.nrb, p.blocks, p.ctas, po, ml);
 }
 template <int BITS, int D>
 static cudaError_t launch(const TreeAttnArgs& a, const Plan& p, cudaStream_t st) {
