@@ -377,6 +377,26 @@ def test_process_logits(dtype, B, T, V, n_bias, mask):
     assert inplace is lg and torch.equal(lg, out) and torch.equal(c2, choice)
 
 
+def test_process_logits_division():
+    """The repetition penalty's quotient is the correctly rounded one: bit for bit torch's fp32 division, for values
+    and penalties of all sizes (subnormal, infinite and zero ones too)."""
+    from myinfer_b200.tree import process_logits
+    g = torch.Generator(device="cuda").manual_seed(2)
+    V = 1 << 16
+    for rep in (1.1, 1.0000001, 1.9999999, 0.3, 3.0, 7.5e-7, 1e30, 1e-38, float("inf")):
+        bits = torch.randint(0, 0x7F800001, (4, V), generator=g, device="cuda", dtype=torch.int32)
+        x = bits.view(torch.float32)
+        x[1] = 30 * torch.rand(V, generator=g, device="cuda")
+        x[2] = torch.randn(V, generator=g, device="cuda").abs() * 2.0 ** -100
+        x[3] = torch.rand(V, generator=g, device="cuda") + 1.0
+        x[0, :3] = torch.tensor([0.0, math.inf, 1.0])
+        counts = torch.ones(4, V, dtype=torch.int32, device="cuda")
+        pen = torch.tensor([[rep, 0.0, 0.0]] * 4, device="cuda")
+        out, _ = process_logits(x, counts=counts, penalties=pen)
+        want = x / pen[:, :1]
+        assert torch.equal(out.nan_to_num(nan=-1.0), want.nan_to_num(nan=-1.0)), rep
+
+
 def test_process_logits_strides_nan_and_ties():
     from myinfer_b200.tree import process_logits
     V = 5003
