@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 from ctypes import c_int64, c_size_t
+from functools import lru_cache
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -32,26 +33,42 @@ from ._lib import M5KvView, M5LayerKv, check, lib
 MAX_NODES = 64
 
 _Kv = Union[torch.Tensor, Sequence[torch.Tensor]]
+_Int64x3 = c_int64 * 3
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a torch.cuda.Stream object costs 2 us
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _launch(name: str, dev: int, *args) -> None:
+    """Call a libm5cuda entry point on device ``dev`` and its current stream (the last argument)."""
+    fn = getattr(lib(), name)
+    if torch._C._cuda_getDevice() == dev:
+        check(fn(*args, _raw_stream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _raw_stream(dev)))
 
 
-def _ints(t: torch.Tensor, shape: tuple, what: str, like: torch.Tensor, dtype=torch.int32) -> int:
-    """Pointer of a contiguous whole-number tensor of this shape on ``like``'s device."""
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != like.device or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {list(shape)} on {like.device}")
+def _whole(t: torch.Tensor, shape: tuple, what: str, dev: int, dtype=torch.int32) -> int:
+    """Pointer of a contiguous tensor of this shape and type on device ``dev``."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {list(shape)} on cuda:{dev}")
     return t.data_ptr()
 
 
 def _tree_shape(parents: torch.Tensor) -> Tuple[int, int]:
-    if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_cuda or not parents.is_contiguous():
+    if parents.dim() != 2 or parents.dtype is not torch.int32 or not parents.is_cuda or not parents.is_contiguous():
         raise ValueError("parents must be a contiguous int32 CUDA tensor [batch, nodes]")
     B, T = parents.shape
     if not 1 <= T <= MAX_NODES:
         raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {T}")
     return B, T
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(dev: int, B: int, Hq: int, Hkv: int, L: int, D: int) -> int:
+    need = c_size_t(0)
+    with torch.cuda.device(dev):
+        check(lib().m5_tree_attention_workspace(B, Hq, Hkv, L, D, ctypes.byref(need)))
+    return need.value
 
 
 def tree_plan(parents: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -62,13 +79,12 @@ def tree_plan(parents: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     B, T = _tree_shape(parents)
     anc = torch.empty(B, T, dtype=torch.int64, device=parents.device)
     depth = torch.empty(B, T, dtype=torch.int32, device=parents.device)
-    with torch.cuda.device(parents.device):
-        check(lib().m5_tree_plan(parents.data_ptr(), B, T, anc.data_ptr(), depth.data_ptr(), _stream(parents)))
+    _launch("m5_tree_plan", parents.get_device(), parents.data_ptr(), B, T, anc.data_ptr(), depth.data_ptr())
     return anc, depth
 
 
-def _kv_parts(t: _Kv, bits: int, D: int, q: torch.Tensor, what: str):
-    """(view, batch, kv heads, rows) of a K or V operand over the whole cache."""
+def _kv_parts(t: _Kv, bits: int, D: int, dev: int, what: str):
+    """(view, [batch, kv heads, rows, width]) of a K or V operand over the whole cache."""
     if bits:
         if isinstance(t, torch.Tensor) or len(t) != 3:
             raise ValueError(f"{what} of a quantized cache are (wq, scales, biases)")
@@ -77,22 +93,24 @@ def _kv_parts(t: _Kv, bits: int, D: int, q: torch.Tensor, what: str):
     else:
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{what} of an unquantized cache are one bf16 tensor")
-        data, s, b, width, dtype = t, None, None, D, torch.bfloat16
-    if data.dim() != 4 or data.dtype != dtype or data.shape[3] != width or data.device != q.device:
-        raise ValueError(f"{what} must be {dtype} [batch, kv heads, rows, {width}] on {q.device}")
-    st = data.stride()
-    if st[3] != 1 or st[2] != width or st[1] % width or st[0] % width:
+        data, width, dtype = t, D, torch.bfloat16
+    shape = data.shape
+    if len(shape) != 4 or data.dtype is not dtype or shape[3] != width or data.get_device() != dev:
+        raise ValueError(f"{what} must be {dtype} [batch, kv heads, rows, {width}] on cuda:{dev}")
+    sb, sh, sr, one = data.stride()
+    if one != 1 or sr != width or sh % width or sb % width:
         raise ValueError(f"{what}: a head's rows must be contiguous")
-    rows_h, rows_b = st[1] // width, st[0] // width
+    rows_b, rows_h = sb // width, sh // width
     if not bits:
-        return M5KvView(data.data_ptr(), None, None, rows_b, rows_h), data.shape
+        return M5KvView(data.data_ptr(), None, None, rows_b, rows_h), shape
     G = D // 64
+    want, lay = (*shape[:3], G), (rows_b * G, rows_h * G, G, 1)
     for x in (s, b):
-        if x.dtype != torch.bfloat16 or x.shape != (*data.shape[:3], G) or x.device != q.device:
-            raise ValueError(f"{what}: scales and biases must be bf16 [batch, kv heads, rows, {G}] on {q.device}")
-        if x.stride() != (rows_b * G, rows_h * G, G, 1):
+        if x.dtype is not torch.bfloat16 or x.shape != want or x.get_device() != dev:
+            raise ValueError(f"{what}: scales and biases must be bf16 [batch, kv heads, rows, {G}] on cuda:{dev}")
+        if x.stride() != lay:
             raise ValueError(f"{what}: scales and biases must be laid out like the rows")
-    return M5KvView(data.data_ptr(), s.data_ptr(), b.data_ptr(), rows_b, rows_h), data.shape
+    return M5KvView(data.data_ptr(), s.data_ptr(), b.data_ptr(), rows_b, rows_h), shape
 
 
 def tree_attention(queries: torch.Tensor, q_keys: _Kv, q_values: _Kv, lengths: torch.Tensor, ancestors: torch.Tensor,
@@ -107,9 +125,10 @@ def tree_attention(queries: torch.Tensor, q_keys: _Kv, q_values: _Kv, lengths: t
     ancestors: int64 [B, L], bit j = the query sees tree key ``lengths[b] + j``;
     ``tree_len`` (default L) is the number of tree keys.  A query that sees no
     key gives zeros.  Returns bf16 [B, Hq, L, D] (``out`` if given)."""
-    if queries.dim() != 4 or queries.dtype != torch.bfloat16 or not queries.is_cuda:
+    if queries.dim() != 4 or queries.dtype is not torch.bfloat16 or not queries.is_cuda:
         raise ValueError("queries must be bf16 CUDA [batch, heads, nodes, dim]")
     B, Hq, L, D = queries.shape
+    dev = queries.get_device()
     T = L if tree_len is None else int(tree_len)
     if D not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {D}")
@@ -117,36 +136,31 @@ def tree_attention(queries: torch.Tensor, q_keys: _Kv, q_values: _Kv, lengths: t
         raise ValueError(f"a tree has 1 to {MAX_NODES} nodes, got {L} queries and {T} tree keys")
     if bits not in (0, 4, 8) or (bits and group_size != 64):
         raise ValueError("tree_attention supports bits 4/8 with group_size 64, or bits 0 (bf16)")
-    kv_k, shape = _kv_parts(q_keys, bits, D, queries, "keys")
-    kv_v, vshape = _kv_parts(q_values, bits, D, queries, "values")
+    kv_k, shape = _kv_parts(q_keys, bits, D, dev, "keys")
+    kv_v, vshape = _kv_parts(q_values, bits, D, dev, "values")
     if shape != vshape or shape[0] != B:
         raise ValueError(f"keys {tuple(shape)} and values {tuple(vshape)} must agree and have batch {B}")
     Hkv, rows = shape[1], shape[2]
     if Hkv == 0 or Hq % Hkv:
         raise ValueError("number of query heads must be a multiple of kv heads")
-    len_p = _ints(lengths, (B,), "lengths", queries)
-    anc_p = _ints(ancestors, (B, L), "ancestors", queries, torch.int64)
+    len_p = _whole(lengths, (B,), "lengths", dev)
+    anc_p = _whole(ancestors, (B, L), "ancestors", dev, torch.int64)
     q = queries
-    qs = q.stride()
-    if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) % 8 or q.data_ptr() % 16:
+    sb, sh, sl, one = q.stride()
+    if one != 1 or (sb | sh | sl) % 8 or q.data_ptr() % 16:
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-        qs = q.stride()
+        sb, sh, sl, one = q.stride()
     if out is None:
         out = torch.empty((B, Hq, L, D), dtype=torch.bfloat16, device=q.device)
-    elif out.shape != queries.shape or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(3) != 1:
+    elif out.shape != queries.shape or out.dtype is not torch.bfloat16 or out.get_device() != dev or out.stride(3) != 1:
         raise ValueError("out must be bf16 of the queries' shape with contiguous dims")
-    os_ = out.stride()
-    L_ = lib()
-    with torch.cuda.device(q.device):
-        need = c_size_t(0)
-        check(L_.m5_tree_attention_workspace(B, Hq, Hkv, L, D, ctypes.byref(need)))
-        # from the stream's own pool: calls on other streams never share it
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-        check(L_.m5_tree_attention(q.data_ptr(), (c_int64 * 3)(*qs[:3]), B, Hq, L, D, kv_k, kv_v, Hkv, rows, len_p, T,
-                                   anc_p, L, float(scale), group_size, bits, out.data_ptr(), (c_int64 * 3)(*os_[:3]),
-                                   None if ws is None else ws.data_ptr(), need.value, _stream(q)))
+    need = _workspace_bytes(dev, B, Hq, Hkv, L, D)
+    # from the stream's own pool: calls on other streams never share it
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _launch("m5_tree_attention", dev, q.data_ptr(), _Int64x3(sb, sh, sl), B, Hq, L, D, kv_k, kv_v, Hkv, rows, len_p, T,
+            anc_p, L, float(scale), group_size, bits, out.data_ptr(), _Int64x3(*out.stride()[:3]), ws.data_ptr(), need)
     return out
 
 
@@ -176,6 +190,7 @@ def process_logits(logits: torch.Tensor, batch: Optional[int] = None, counts: Op
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or not logits.is_cuda:
         raise ValueError("logits must be bf16 or fp32 CUDA [rows, vocab]")
     R, V = logits.shape
+    dev = logits.get_device()
     B = R if batch is None else int(batch)
     if B < 1 or R % B:
         raise ValueError(f"{R} logits rows are no multiple of batch {batch}")
@@ -192,26 +207,25 @@ def process_logits(logits: torch.Tensor, batch: Optional[int] = None, counts: Op
         raise ValueError("counts and tokens need penalties")
     if (tokens is None) != (ancestors is None) or (bias_ids is None) != (bias_values is None):
         raise ValueError("tokens come with ancestors, and bias_ids with bias_values")
-    cp = None if counts is None else _ints(counts, (B, V), "counts", logits)
-    pp = None if penalties is None else _ints(penalties, (B, 3), "penalties", logits, torch.float32)
-    tp = None if tokens is None else _ints(tokens, (B, T), "tokens", logits)
-    ap = None if ancestors is None else _ints(ancestors, (B, T), "ancestors", logits, torch.int64)
+    cp = None if counts is None else _whole(counts, (B, V), "counts", dev)
+    pp = None if penalties is None else _whole(penalties, (B, 3), "penalties", dev, torch.float32)
+    tp = None if tokens is None else _whole(tokens, (B, T), "tokens", dev)
+    ap = None if ancestors is None else _whole(ancestors, (B, T), "ancestors", dev, torch.int64)
     nb, ip, vp = 0, None, None
     if bias_ids is not None:
         nb = bias_ids.shape[-1]
-        ip = _ints(bias_ids, (B, nb), "bias_ids", logits)
-        vp = _ints(bias_values, (B, nb), "bias_values", logits, torch.float32)
+        ip = _whole(bias_ids, (B, nb), "bias_ids", dev)
+        vp = _whole(bias_values, (B, nb), "bias_values", dev, torch.float32)
     mp, mld = None, 0
     if mask is not None:
         mld = mask.shape[-1]
-        mp = _ints(mask, (R, mld), "mask", logits)
+        mp = _whole(mask, (R, mld), "mask", dev)
     choices = torch.empty(R, dtype=torch.int32, device=logits.device)
     # a single row's stride is meaningless (torch keeps any stride on a size-1 dimension)
     ld, old = (logits.stride(0), out.stride(0)) if R > 1 else (V, V)
-    dt = _lib.M5_DTYPE_BF16 if logits.dtype == torch.bfloat16 else _lib.M5_DTYPE_F32
-    with torch.cuda.device(logits.device):
-        check(lib().m5_process_logits(logits.data_ptr(), ld, out.data_ptr(), old, dt, B, T, V, cp, V, pp, tp, ap, ip,
-                                      vp, nb, mp, mld, choices.data_ptr(), _stream(logits)))
+    dt = _lib.M5_DTYPE_BF16 if logits.dtype is torch.bfloat16 else _lib.M5_DTYPE_F32
+    _launch("m5_process_logits", dev, logits.data_ptr(), ld, out.data_ptr(), old, dt, B, T, V, cp, V, pp, tp, ap, ip, vp,
+            nb, mp, mld, choices.data_ptr())
     return out, choices
 
 
@@ -224,19 +238,18 @@ def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, picks: torch.Tensor
     ``counts`` (int32 [B, V], see ``process_logits``) gains 1 for every accepted
     node's token."""
     B, T = _tree_shape(parents)
-    tp = _ints(tokens, (B, T), "tokens", parents)
-    pp = _ints(picks, (B, T), "picks", parents)
+    dev = parents.get_device()
+    tp = _whole(tokens, (B, T), "tokens", dev)
+    pp = _whole(picks, (B, T), "picks", dev)
     cp, V = None, 0
     if counts is not None:
         if counts.dim() != 2:
             raise ValueError("counts must be int32 [batch, vocab]")
         V = counts.shape[1]
-        cp = _ints(counts, (B, V), "counts", parents)
-    o = torch.empty(B * (T + 2), dtype=torch.int32, device=parents.device)
-    path, n, nxt = o[:B * T].view(B, T), o[B * T:B * T + B], o[B * T + B:]
-    with torch.cuda.device(parents.device):
-        check(lib().m5_tree_accept(parents.data_ptr(), tp, pp, B, T, path.data_ptr(), n.data_ptr(), nxt.data_ptr(),
-                                   cp, V, V, _stream(parents)))
+        cp = _whole(counts, (B, V), "counts", dev)
+    path = torch.empty((B, T), dtype=torch.int32, device=parents.device)
+    n, nxt = torch.empty((2, B), dtype=torch.int32, device=parents.device).unbind(0)
+    _launch("m5_tree_accept", dev, parents.data_ptr(), tp, pp, B, T, path.data_ptr(), n.data_ptr(), nxt.data_ptr(), cp, V, V)
     return path, n, nxt
 
 
@@ -249,7 +262,7 @@ class CacheLayers:
         pairs: List[tuple] = [(c.keys, c.values) if hasattr(c, "keys") else tuple(c) for c in layers]
         if not pairs:
             raise ValueError("no cache layers")
-        self._keep = pairs
+        self._keep = pairs  # the table holds addresses only
         arr = (M5LayerKv * len(pairs))()
         shape = None
         for a, (k, v) in zip(arr, pairs):
@@ -295,10 +308,7 @@ def commit_tree(layers, lengths: torch.Tensor, path: torch.Tensor, accepted: tor
     if path.dim() != 2 or path.shape[0] != t.batch or not 1 <= path.shape[1] <= MAX_NODES:
         raise ValueError(f"path must be int32 [{t.batch}, 1 to {MAX_NODES} nodes]")
     B, T = path.shape
-    like = t._keep[0][0] if isinstance(t._keep[0][0], torch.Tensor) else t._keep[0][0][0]
-    pp = _ints(path, (B, T), "path", like)
-    lp = _ints(lengths, (B,), "lengths", like)
-    np_ = _ints(accepted, (B,), "accepted", like)
-    with torch.cuda.device(t.device):
-        check(lib().m5_tree_commit(t.structs, len(t.structs), B, t.kv_heads, t.head_dim, lp, pp, T, np_,
-                                   _stream(like)))
+    dev = t.device.index
+    _launch("m5_tree_commit", dev, t.structs, len(t.structs), B, t.kv_heads, t.head_dim,
+            _whole(lengths, (B,), "lengths", dev), _whole(path, (B, T), "path", dev), T,
+            _whole(accepted, (B,), "accepted", dev))
