@@ -251,6 +251,17 @@ typedef struct m5_sample_params {
 M5_API int m5_sample_bf16(void* logits, int rows, int64_t vocab, int64_t ld, int32_t* history, int hist_len,
                           int64_t hist_ld, const m5_sample_params* p, uint64_t* state, int32_t* out, void* stream);
 
+/* One model call for L nodes of a token tree over a batch-1 cache: node i sits
+ * at position *d_len + d_depths[i], its K/V go to cache row *d_len + row0 + i,
+ * and it attends to the *d_len committed rows and to the tree rows whose bits
+ * are set in d_ancestors[i] (see m5_tree_attention; row0 > 0 extends a tree
+ * whose first row0 nodes are in the cache).  *d_len is left as it is: accept
+ * a path (m5_tree_accept, m5_tree_commit), then advance it.  row0 + L <= 64.
+ * logits as in m5_forward.  The first call on a model allocates its workspace. */
+M5_API int m5_forward_tree(void* model, const m5_layer_kv* kv, int32_t* d_len, const int32_t* d_tokens, int L,
+                           int row0, const int32_t* d_depths, const int64_t* d_ancestors, void* logits,
+                           int logits_mode, void* stream);
+
 /* ------------------------------------------------- speculative token trees
  * Operators of speculative decoding over a tree of drafted tokens (no
  * counterpart in the reference, whose speculation is a single chain).  A

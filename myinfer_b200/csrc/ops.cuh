@@ -23,6 +23,8 @@ struct RopeAppendArgs {
   m5_layer_kv kv;
   int batch;              // > 1: token t is sequence t (L == batch), all at position *d_len;
                           // kv holds [batch, Hkv, capacity, ...]
+  const int32_t* depth;   // nodes of a token tree: token t sits at position *d_len + depth[t] and its
+  int row0;               // K/V go to cache row *d_len + row0 + t (null: position and row *d_len + t)
 };
 int rope_append_launch(const RopeAppendArgs& a, cudaStream_t stream);
 

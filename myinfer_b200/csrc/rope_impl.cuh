@@ -59,7 +59,8 @@ __device__ __forceinline__ void rope_append_row(const RopeAppendArgs& a, int t, 
   constexpr int D = 128;
   const int H3 = a.Hq + 2 * a.Hkv;
   const bool batched = a.batch > 1;
-  const int pos = *a.d_len + (batched ? 0 : t);
+  const int base = *a.d_len;
+  const int pos = base + (a.depth ? a.depth[t] : batched ? 0 : t);
   const uint2* src = reinterpret_cast<const uint2*>(a.qkv + (size_t(t) * H3 + h) * D + 4 * lane);
   const uint2 raw = CG ? __ldcg(src) : *src;
   float x[4] = {bf16_lo(raw.x), bf16_hi(raw.x), bf16_lo(raw.y), bf16_hi(raw.y)};
@@ -100,9 +101,10 @@ __device__ __forceinline__ void rope_append_row(const RopeAppendArgs& a, int t, 
     reinterpret_cast<uint2*>(a.q_out + qrow * D)[lane] = v;
     return;
   }
-  if (pos >= a.kv.capacity) return;  // the host checks capacity; never write past it
+  const int at = base + (a.depth ? a.row0 + t : batched ? 0 : t);
+  if (at >= a.kv.capacity) return;  // the host checks capacity; never write past it
   const int kh = is_k ? h - a.Hq : h - a.Hq - a.Hkv;
-  const size_t row = (size_t(batched ? t : 0) * a.Hkv + kh) * a.kv.capacity + pos;
+  const size_t row = (size_t(batched ? t : 0) * a.Hkv + kh) * a.kv.capacity + at;
   if (is_k) store_kv_row<BITS>(x, lane, a.kv.k, (bf16*)a.kv.k_scales, (bf16*)a.kv.k_biases, row);
   else store_kv_row<BITS>(x, lane, a.kv.v, (bf16*)a.kv.v_scales, (bf16*)a.kv.v_biases, row);
 }

@@ -62,6 +62,8 @@ struct Model {
   int32_t* rids = nullptr;
   float* attn_part = nullptr;
   size_t attn_part_bytes = 0;
+  void* tree_ws = nullptr;  // workspace of the tree attention, made by the first m5_forward_tree
+  size_t tree_ws_bytes = 0;
   void* argmax_scratch = nullptr;
   float* mma_acc = nullptr;  // zeroed split-tile scratch of the tensor-core GEMV
   int* mma_cnt = nullptr;
@@ -449,8 +451,14 @@ static bool stream_capturing(cudaStream_t st) {
 // One model call: L tokens of one sequence at positions *d_len.., or (B > 1,
 // L == 1) one token of each of B sequences, all at position *d_len, over a
 // cache of [B, Hkv, capacity, ...] layers.  T = L * B activation rows.
+// tree: the L tokens are nodes of a token tree (m5_forward_tree); *d_len stays.
+struct TreeCall {
+  const int32_t* depths;
+  const unsigned long long* ancestors;
+  int row0;
+};
 static int forward(Model* m, const m5_layer_kv* kv, int32_t* d_len, const int32_t* d_tokens, int L, void* logits,
-                   int logits_mode, int32_t* d_argmax, cudaStream_t st, int B = 1) {
+                   int logits_mode, int32_t* d_argmax, cudaStream_t st, int B = 1, const TreeCall* tree = nullptr) {
   const int T = L * B;
   const m5_model_cfg& c = m->cfg;
   const int H = c.hidden_size, D = c.head_dim;
@@ -490,6 +498,10 @@ static int forward(Model* m, const m5_layer_kv* kv, int32_t* d_len, const int32_
     r.d_len = d_len;
     r.q_out = m->q;
     r.kv = lk;
+    if (tree) {
+      r.depth = tree->depths;
+      r.row0 = tree->row0;
+    }
     if (T < kGemmMinRows && T <= 8 && D == 128 && fuse_rope() && gemv_tmap_eligible(a, T, EPI_STORE)) {
       // one launch: the GEMV's epilogue appends each head once its rows are written
       a.rope = r;
@@ -499,28 +511,53 @@ static int forward(Model* m, const m5_layer_kv* kv, int32_t* d_len, const int32_
       if ((rc = linear_auto(m, a, T, EPI_STORE, st))) return rc;
       if ((rc = rope_append_launch(r, st))) return rc;
     }
-    // attention over the cache (S = *d_len + L keys after the append)
+    // attention over the cache (S = *d_len + L keys after the append), or of a tree's nodes
     AttnArgs at{};
-    at.q = m->q;
-    at.B = B;
-    at.Hq = Hq;
-    at.L = L;
-    at.D = D;
-    at.k = m5_kv_view{lk.k, lk.k_scales, lk.k_biases, int64_t(Hkv) * lk.capacity, lk.capacity};
-    at.v = m5_kv_view{lk.v, lk.v_scales, lk.v_biases, int64_t(Hkv) * lk.capacity, lk.capacity};
-    at.bits = lk.bits;
-    at.Hkv = Hkv;
-    at.d_S = d_len;
-    at.S_add = L;
-    at.scale = 1.f / sqrtf(float(D));
-    at.mask_kind = L > 1 ? M5_MASK_CAUSAL : M5_MASK_NONE;
-    attn_plan(B, Hq, Hkv, L, (int)lk.capacity, at.QB, at.nsplit);
-    if (attn_scratch_bytes(B, Hq, L, D, at.nsplit) > m->attn_part_bytes) at.nsplit = 1;
-    at.part_o = m->attn_part;
-    at.part_ml = m->attn_part + size_t(B) * Hq * L * at.nsplit * D;
-    at.out = m->attn;
-    at.out_tokens_major = 1;
-    if ((rc = attn_launch(at, st))) return rc;
+    if (tree) {
+      TreeAttnArgs ta{};
+      ta.q = m->q;  // [Hq, L, D]
+      ta.q_sh = int64_t(L) * D;
+      ta.q_sl = D;
+      ta.out = m->attn;  // [L, Hq, D]
+      ta.o_sh = D;
+      ta.o_sl = int64_t(Hq) * D;
+      ta.B = 1;
+      ta.Hq = Hq;
+      ta.Hkv = Hkv;
+      ta.L = L;
+      ta.T = tree->row0 + L;
+      ta.D = D;
+      ta.bits = lk.bits;
+      ta.k = m5_kv_view{lk.k, lk.k_scales, lk.k_biases, 0, lk.capacity};
+      ta.v = m5_kv_view{lk.v, lk.v_scales, lk.v_biases, 0, lk.capacity};
+      ta.capacity = lk.capacity;
+      ta.lengths = d_len;
+      ta.anc = tree->ancestors;
+      ta.scale = 1.f / sqrtf(float(D));
+      ta.ws = m->tree_ws;
+      if ((rc = tree_attn_check(ta)) || (rc = tree_attn_launch(ta, st))) return rc;
+    } else {
+      at.q = m->q;
+      at.B = B;
+      at.Hq = Hq;
+      at.L = L;
+      at.D = D;
+      at.k = m5_kv_view{lk.k, lk.k_scales, lk.k_biases, int64_t(Hkv) * lk.capacity, lk.capacity};
+      at.v = m5_kv_view{lk.v, lk.v_scales, lk.v_biases, int64_t(Hkv) * lk.capacity, lk.capacity};
+      at.bits = lk.bits;
+      at.Hkv = Hkv;
+      at.d_S = d_len;
+      at.S_add = L;
+      at.scale = 1.f / sqrtf(float(D));
+      at.mask_kind = L > 1 ? M5_MASK_CAUSAL : M5_MASK_NONE;
+      attn_plan(B, Hq, Hkv, L, (int)lk.capacity, at.QB, at.nsplit);
+      if (attn_scratch_bytes(B, Hq, L, D, at.nsplit) > m->attn_part_bytes) at.nsplit = 1;
+      at.part_o = m->attn_part;
+      at.part_ml = m->attn_part + size_t(B) * Hq * L * at.nsplit * D;
+      at.out = m->attn;
+      at.out_tokens_major = 1;
+      if ((rc = attn_launch(at, st))) return rc;
+    }
     // o_proj, residual add into h
     GemvArgs o{};
     o.x = m->attn;
@@ -642,7 +679,7 @@ static int forward(Model* m, const m5_layer_kv* kv, int32_t* d_len, const int32_
   if (d_argmax && last_row) {
     if ((rc = argmax_launch(last_row, V, d_argmax, m->argmax_scratch, st))) return rc;
   }
-  M5_CUDA(launch_pdl(add_len_kernel, dim3(1), dim3(1), 0, st, d_len, L));
+  if (!tree) M5_CUDA(launch_pdl(add_len_kernel, dim3(1), dim3(1), 0, st, d_len, L));
   return M5_OK;
 }
 
@@ -896,6 +933,7 @@ extern "C" int m5_model_destroy(void* model) {
   Model* m = (Model*)model;
   if (!m) return M5_OK;
   if (m->arena) cudaFree(m->arena);
+  if (m->tree_ws) cudaFree(m->tree_ws);
   if (m->d_inv_freq) cudaFree(m->d_inv_freq);
   if (m->h_moe_cnt) cudaFreeHost(m->h_moe_cnt);
   for (int i = 0; i < Model::kMoeStreams; ++i) {
@@ -1088,6 +1126,25 @@ extern "C" int m5_forward(void* model, const m5_layer_kv* kv, int32_t* d_len, co
   Model* m = (Model*)model;
   if (int rc = check_forward(m, kv, L, logits_mode, logits, "m5_forward")) return rc;
   return forward(m, kv, d_len, d_tokens, L, logits, logits_mode, d_argmax, (cudaStream_t)stream);
+}
+
+extern "C" int m5_forward_tree(void* model, const m5_layer_kv* kv, int32_t* d_len, const int32_t* d_tokens, int L,
+                               int row0, const int32_t* d_depths, const int64_t* d_ancestors, void* logits,
+                               int logits_mode, void* stream) {
+  M5_CHECK_ARG(model && kv && d_len && d_tokens && d_depths && d_ancestors, "m5_forward_tree: null argument");
+  M5_CHECK_ARG(L > 0 && row0 >= 0, "m5_forward_tree: L must be positive and row0 not negative");
+  M5_CHECK_ARG(L <= kTreeMax && row0 <= kTreeMax - L, "m5_forward_tree: more than 64 nodes");
+  Model* m = (Model*)model;
+  if (int rc = check_forward(m, kv, L, logits_mode, logits, "m5_forward_tree")) return rc;
+  const size_t need = tree_attn_ws_bytes(1, m->Hq, m->Hkv, kTreeMax, m->cfg.head_dim);
+  if (m->tree_ws_bytes < need) {
+    if (stream_capturing((cudaStream_t)stream))
+      return fail(M5_ERR_STATE, "m5_forward_tree: the first call allocates its workspace and cannot be captured");
+    M5_CUDA(cudaMalloc(&m->tree_ws, need));
+    m->tree_ws_bytes = need;
+  }
+  const TreeCall t{d_depths, (const unsigned long long*)d_ancestors, row0};
+  return forward(m, kv, d_len, d_tokens, L, logits, logits_mode, nullptr, (cudaStream_t)stream, 1, &t);
 }
 
 extern "C" int m5_forward_batch(void* model, const m5_layer_kv* kv, int32_t* d_len, const int32_t* d_tokens, int B,

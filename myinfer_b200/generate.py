@@ -34,6 +34,7 @@ from . import _lib
 from .attention import safe_maybe_quantize_kv_cache
 from .cache import PromptCache, make_prompt_cache, trim_prompt_cache
 from .sample import DeviceSampler, with_processors
+from .tree import MAX_NODES, CacheLayers, commit_tree, process_logits, tree_accept, tree_plan
 
 STATUS_EVERY = 64  # decode steps between reads of the device error words
 
@@ -327,11 +328,148 @@ def speculative_generate_step(prompt: List[int], model, draft_model, num_draft_t
         stats["decode_time"] = time.perf_counter() - t1
 
 
+def tree_shape(widths) -> List[List[int]]:
+    """Parents of each level's nodes in a tree whose nodes at depth d all have
+    ``widths[d]`` children: [[-1], [0] * w0, ...], numbered level by level."""
+    widths = [int(w) for w in widths]
+    if not widths or min(widths) < 1:
+        raise ValueError(f"tree_widths must be positive, got {widths}")
+    levels, n = [[-1]], 1
+    for w in widths:
+        first = n - len(levels[-1])
+        levels.append([first + i for i in range(len(levels[-1])) for _ in range(w)])
+        n += len(levels[-1])
+        if n > MAX_NODES:
+            raise ValueError(f"tree_widths {widths} make more than {MAX_NODES} nodes")
+    return levels
+
+
+def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_widths=(4, 2, 1, 1),
+                                   max_tokens: int = 256, sampler: Optional[DeviceSampler] = None,
+                                   penalties: Optional[tuple] = None, logit_bias: Optional[dict] = None,
+                                   grammar: Optional[Callable] = None, prompt_cache: Optional[PromptCache] = None,
+                                   draft_cache: Optional[PromptCache] = None, prefill_step_size: int = 2048,
+                                   kv_bits: Optional[int] = None, kv_group_size: int = 64,
+                                   quantized_kv_start: int = 0, stats: Optional[dict] = None) -> Iterator[tuple]:
+    """Speculative decoding over a tree of drafts: each round the draft model
+    proposes, for every node of a level, its ``tree_widths[d]`` likeliest tokens,
+    the main model scores all nodes in one call, and the longest path whose
+    tokens equal the main model's own choices is kept (``myinfer_b200.tree``).
+    With widths of 1 this is the chain of ``speculative_generate_step``; wider
+    levels accept more tokens per call for the same number of draft calls.
+    Yields (token, from_draft); greedy tokens equal the main model's greedy
+    decode (with the same processors).
+
+    ``sampler``: a ``DeviceSampler`` draws the choices from the processed logits
+    (its own penalty window is not used).  ``penalties`` = (repetition, presence,
+    frequency) over the whole context; ``logit_bias`` maps token ids to added
+    values; ``grammar(tokens, nodes, parents)`` returns the int32 bit mask
+    [len(nodes), ceil(V / 32)] on the device for the tokens that may follow each
+    node (``tokens``: everything before the tree, ``nodes``: the nodes' tokens) or None."""
+    if not prompt:
+        raise ValueError("empty prompt")
+    V = model.args.vocab_size
+    if draft_model.args.vocab_size != V:
+        raise ValueError("draft model vocabulary differs from the main model's")
+    if min(prompt) < 0 or max(prompt) >= V:
+        raise ValueError(f"token id out of range [0, {V})")
+    if sampler is not None and not isinstance(sampler, DeviceSampler):
+        raise ValueError("tree speculation samples with a DeviceSampler (make_sampler) or greedily")
+    if sampler is not None and sampler.window:
+        raise ValueError("give penalties to tree speculation itself: a node's window is its own path")
+    levels = tree_shape(tree_widths)
+    T = sum(len(lv) for lv in levels)
+    dev = model.device
+    mcache = prompt_cache if prompt_cache is not None else make_prompt_cache(model)
+    dcache = draft_cache if draft_cache is not None else make_prompt_cache(draft_model)
+    if mcache.offset != dcache.offset:
+        raise ValueError("the two caches hold different lengths")
+    prompt_t = torch.as_tensor(prompt, dtype=torch.int32).to(dev)
+    parents = torch.tensor([[p for lv in levels for p in lv]], dtype=torch.int32).to(dev)
+    ancestors, depths = tree_plan(parents)
+    total = mcache.offset + len(prompt) + max_tokens + T
+    for m in (model, draft_model):
+        m.reserve(max(T, min(prefill_step_size, max(1, len(prompt) - 1))))
+    for m, cache in ((model, mcache), (draft_model, dcache)):
+        for p0 in range(0, len(prompt) - 1, prefill_step_size):
+            m.forward(prompt_t[p0:min(p0 + prefill_step_size, len(prompt) - 1)], cache)
+            safe_maybe_quantize_kv_cache(cache, quantized_kv_start, kv_group_size, kv_bits)
+        for c in cache:
+            c.reserve(total)
+    counts = pen = ids = values = None
+    if penalties is not None:
+        pen = torch.tensor([list(penalties)], dtype=torch.float32).to(dev)
+        counts = torch.bincount(prompt_t[:-1].long(), minlength=V).to(torch.int32)[None].contiguous()
+    if logit_bias:
+        ids = torch.tensor([list(logit_bias)], dtype=torch.int32).to(dev)
+        values = torch.tensor([list(logit_bias.values())], dtype=torch.float32).to(dev)
+    tokens = torch.zeros(1, T, dtype=torch.int32, device=dev)
+    tokens[0, 0] = prompt_t[-1]
+    logits = torch.empty(T, V, dtype=torch.bfloat16, device=dev)
+    d_logits = torch.empty(max(len(lv) for lv in levels), V, dtype=torch.bfloat16, device=dev)
+    lengths = torch.zeros(1, dtype=torch.int32, device=dev)
+    seen = list(prompt[:-1])
+    tables, sig = None, None
+    ntoks = 0
+    if stats is not None:
+        stats["prompt_tokens"] = len(prompt)
+    t1 = time.perf_counter()
+    while ntoks < max_tokens:
+        # draft level by level; the last level's nodes only leave their keys and values
+        row0 = 0
+        for lv, w in zip(levels, list(tree_widths) + [0]):
+            row1 = row0 + len(lv)
+            node = slice(row0, row1)
+            lg = d_logits[:len(lv)] if w else None
+            draft_model.forward_tree(tokens[0, node], dcache, depths[0, node], ancestors[0, node], row0,
+                                     _lib.M5_LOGITS_ALL if w else _lib.M5_LOGITS_NONE, lg)
+            if w:
+                tokens[0, row1:row1 + len(lv) * w] = lg.float().topk(w, dim=-1).indices.reshape(-1).to(torch.int32)
+            row0 = row1
+        model.forward_tree(tokens[0], mcache, depths[0], ancestors[0], 0, _lib.M5_LOGITS_ALL, logits)
+        for cache in (mcache, dcache):
+            safe_maybe_quantize_kv_cache(cache, quantized_kv_start, kv_group_size, kv_bits)
+        mask = None if grammar is None else grammar(seen, tokens[0].tolist(), parents[0].tolist())
+        _, picks = process_logits(logits, batch=1, counts=counts, penalties=pen,
+                                  tokens=None if pen is None else tokens, ancestors=None if pen is None else ancestors,
+                                  bias_ids=ids, bias_values=values, mask=mask, out=logits)
+        if sampler is not None:
+            logits[:, 0] = torch.where(picks < 0, 0.0, logits[:, 0])  # the sampler takes no row of -inf's alone
+            picks = torch.where(picks < 0, picks, sampler(logits))    # a node the grammar leaves nothing stays -1
+        path, n, nxt = tree_accept(parents, tokens, picks.reshape(1, T), counts=counts)
+        if sig != (mcache.signature(), dcache.signature()):
+            tables, sig = (CacheLayers(mcache), CacheLayers(dcache)), (mcache.signature(), dcache.signature())
+        lengths.fill_(mcache.offset)
+        for t in tables:
+            commit_tree(t, lengths, path, n)
+        host = torch.cat([tokens[0], path[0], n, nxt]).tolist()  # one host sync per round
+        k, y = host[2 * T], host[2 * T + 1]
+        kept = [host[i] for i in host[T:T + k]]
+        for cache in (mcache, dcache):
+            for c in cache:
+                c.offset += k
+        _lib.device_check()
+        seen += kept
+        for t in kept[1:]:
+            ntoks += 1
+            yield t, True
+            if ntoks == max_tokens:
+                break
+        if ntoks == max_tokens or y < 0:  # y < 0: the grammar allows no token here
+            break
+        ntoks += 1
+        yield y, False
+        tokens[0, 0] = y
+    if stats is not None:
+        stats["decode_time"] = time.perf_counter() - t1
+
+
 def stream_generate(model, tokenizer, prompt, max_tokens: int = 256, draft_model=None,
                     **kwargs) -> Iterator[GenerationResponse]:
     """mlx-lm ``stream_generate`` surface used by the engine (greedy or sampler;
     speculative decoding when ``draft_model`` is given: ``num_draft_tokens`` and
-    ``draft_cache`` are then read from the keyword arguments)."""
+    ``draft_cache`` are then read from the keyword arguments; ``tree_widths``
+    drafts a tree instead of a chain)."""
     if isinstance(prompt, str):
         prompt = tokenizer.encode(prompt)
     prompt = [int(t) for t in (prompt.tolist() if hasattr(prompt, "tolist") else prompt)]
@@ -341,10 +479,15 @@ def stream_generate(model, tokenizer, prompt, max_tokens: int = 256, draft_model
     n = 0
     if draft_model is not None:
         kwargs.pop("use_graph", None)
-        steps = speculative_generate_step(prompt, model, draft_model, max_tokens=max_tokens, stats=stats, **kwargs)
+        if kwargs.get("tree_widths"):
+            kwargs.pop("num_draft_tokens", None)
+            steps = tree_speculative_generate_step(prompt, model, draft_model, max_tokens=max_tokens, stats=stats, **kwargs)
+        else:
+            kwargs.pop("tree_widths", None)
+            steps = speculative_generate_step(prompt, model, draft_model, max_tokens=max_tokens, stats=stats, **kwargs)
     else:
-        kwargs.pop("num_draft_tokens", None)
-        kwargs.pop("draft_cache", None)
+        for k in ("num_draft_tokens", "draft_cache", "tree_widths"):
+            kwargs.pop(k, None)
         steps = ((t, False) for t, _ in generate_step(prompt, model, max_tokens, stats=stats, **kwargs))
     for token, from_draft in steps:
         n += 1

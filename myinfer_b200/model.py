@@ -274,6 +274,30 @@ class Model:
         for c in cache:
             c.offset += L
 
+    def forward_tree(self, tokens: torch.Tensor, cache: PromptCache, depths: torch.Tensor, ancestors: torch.Tensor,
+                     row0: int = 0, logits_mode: int = _lib.M5_LOGITS_NONE,
+                     logits: Optional[torch.Tensor] = None) -> None:
+        """Run L nodes of a token tree (int32 CUDA tokens and depths [L], int64
+        ancestor words [L] as ``tree.tree_plan`` makes them) behind the cache's
+        committed rows: node i goes to row ``cache.offset + row0 + i``.  The
+        offset stays; accept a path with ``tree.tree_accept`` and
+        ``tree.commit_tree``, then add its length to every layer's offset."""
+        L = int(tokens.numel())
+        for t, dt, what in ((tokens, torch.int32, "tokens"), (depths, torch.int32, "depths"),
+                            (ancestors, torch.int64, "ancestors")):
+            if t.dtype is not dt or t.numel() != L or not t.is_cuda or not t.is_contiguous():
+                raise ValueError(f"forward_tree: {what} must be {L} contiguous {dt} values on the device")
+        if L > self.max_tokens:
+            self.reserve(L)
+        need = cache.offset + row0 + L
+        for c in cache:
+            if c.capacity < need:
+                c.reserve(need)
+        cache.d_len.fill_(cache.offset)
+        call("m5_forward_tree", self._h, cache.structs(), cache.d_len.data_ptr(), tokens.data_ptr(), L, int(row0),
+             depths.data_ptr(), ancestors.data_ptr(), None if logits is None else logits.data_ptr(), logits_mode,
+             _stream())
+
     def prefill_sequence(self, tokens: torch.Tensor, cache: PromptCache, seq: int, chunk: int = 2048) -> None:
         """Prefill sequence `seq` of a batched cache with `tokens` (int32 CUDA
         [L]) from position 0, in chunks; the cache's shared offset is left to
