@@ -14,8 +14,8 @@
 //
 // Roles of a CTA (896 threads, registers moved to the softmax by setmaxnreg):
 //   warp 25      producer: bulk copies of 64-key tiles of K / V rows and of their
-//                scales and biases (as the 16-byte blocks around them, so any
-//                2-byte alignment will do) into a ring;
+//                scales and biases (as the 16-byte blocks around them, since a head's may
+//                start anywhere) into a ring;
 //   warps 26-27  scales, even and odd tiles: per tile and operand the exponent that puts the tile's largest value
 //                under 2^-2, and scale and bias in fp16 under it;
 //   warps 16-23  conversion to fp16, four warps for K and four for V, both into [key][dim] rows of
@@ -41,6 +41,7 @@
 // TMEM columns: S / P [stream][2] 64 each, O [stream] 128 each.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "tcgen05.cuh"
 #include "tree.cuh"
@@ -56,9 +57,6 @@ constexpr int ROWS = 128;   // MMA M
 constexpr int SMX_WARPS = 16, DQ_WARPS = 4;  // conversion: DQ_WARPS for K and as many for V
 constexpr int MMA_WARP = SMX_WARPS + 2 * DQ_WARPS, PROD_WARP = MMA_WARP + 1, PREP_WARP = MMA_WARP + 2;
 constexpr int THREADS = (PREP_WARP + 2) * 32;
-// registers per thread after setmaxnreg: 4 + 2 + 1 warpgroups out of 896 x 72 at launch
-constexpr int SMX_REGS = 80, DQ_REGS = 72, MISC_REGS = 40;
-static_assert(512 * SMX_REGS + 256 * DQ_REGS + 128 * MISC_REGS <= 896 * 72, "register split");
 constexpr int EXPS = 32;    // tile exponents held: more than the tiles between conversion and softmax
 constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -79,13 +77,17 @@ struct Cfg {
   static constexpr int SWIN = BITS ? TK * 2 * G + 32 : 0;       // a tile's scales with the 16-byte blocks around them
   static constexpr int K_OFF = 0, V_OFF = TK * KROW;
   static constexpr int S_OFF = 2 * TK * KROW;                   // K scales, K biases, V scales, V biases
-  static constexpr int H_OFF = S_OFF + 4 * SWIN;                // fp16 (s, s), (b, b) per key and group, K then V
+  static constexpr int H_OFF = (S_OFF + 4 * SWIN + 15) / 16 * 16;                // fp16 (s, s), (b, b) per key and group, K then V
   static constexpr int STAGE = (H_OFF + (BITS ? 2 * TK * G * 8 : 0) + 127) / 128 * 128;
   static constexpr int OPER = TK * D * 2;                       // a converted tile
   static constexpr int NOP = TWO && BITS == 0 && D == 128 ? 2 : 3;  // converted K and V tiles held
   static constexpr int CW = BITS ? DQ_WARPS / 2 : DQ_WARPS;     // conversion warps per tile and operand
   static constexpr int BLOCKS = TWO ? 2 : 1;
   static constexpr int QBLOCK = ROWS * D * 2, QBYTES = BLOCKS * QBLOCK;
+  // registers per thread after setmaxnreg: 4 + 2 + 1 warpgroups out of 896 x 72 at launch.  A spill
+  // in the single warps costs most, it is on every tile's path.
+  static constexpr int SMX_REGS = 80, DQ_REGS = BITS ? 56 : 64, MISC_REGS = BITS ? 72 : 56;
+  static_assert(512 * SMX_REGS + 256 * DQ_REGS + 128 * MISC_REGS <= THREADS * 72, "register split");
   static constexpr int FIXED = QBYTES + 2 * NOP * OPER + 1024 + 1024;  // + alignment, barriers
   static constexpr int ST = (227 * 1024 - 6656 - FIXED) / STAGE < 8 ? (227 * 1024 - 6656 - FIXED) / STAGE : 8;
   static constexpr int SMEM = FIXED + ST * STAGE;
@@ -485,107 +487,118 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
   const uint32_t tmem = s_tmem;
   const Line line = s_line;
 
-  if (warp >= MMA_WARP) setmaxnreg_dec<MISC_REGS>();
+  if (warp >= MMA_WARP) setmaxnreg_dec<C::MISC_REGS>();
   if (warp == PROD_WARP) {
     // ------------------------------------------------------------- producer
-    if (lane == 0) {
-      Walk w(line, a);
-      Slot<ST> r;
-      int issued = 0;
-      bool ok = true;
-      while (ok && w.next(a, nrb)) {
-        int64_t kr = w.b * a.k.batch_stride + w.hk * a.k.head_stride + w.t0 * TK;  // row of the tile's first key
-        int64_t vr = w.b * a.v.batch_stride + w.hk * a.v.head_stride + w.t0 * TK;
-        int left = w.kend - w.t0 * TK;  // keys from the tile on
+    // Lanes 0 and 1 copy the tile's K and V rows, lanes 2-5 the 16-byte blocks that hold its K
+    // scales, K biases, V scales and V biases: each works out its own copy.
+    constexpr int COPIES = BITS ? 6 : 2;
+    const int op = lane < 2 ? lane : (lane - 2) >> 1;  // K, V
+    const m5_kv_view& view = op ? a.v : a.k;
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(lane < 2 ? view.data : (lane & 1) ? view.biases : view.scales);
+    const int unit = lane < 2 ? C::KROW : C::SROW;     // bytes per key
+    const int to = lane < 2 ? (op ? C::V_OFF : C::K_OFF) : C::S_OFF + (lane - 2) * C::SWIN;
+    Walk w(line, a);
+    Slot<ST> r;
+    int issued = 0;
+    bool ok = true;
+    while (ok && w.next(a, nrb)) {
+      int left = w.kend - w.t0 * TK;  // keys from the tile on
+      const uint8_t* from = src + (w.b * view.batch_stride + w.hk * view.head_stride + w.t0 * TK) * unit;
 #pragma unroll 1
-        for (int t = 0; t < w.nt; ++t, kr += TK, vr += TK, left -= TK) {
-          const int nk = min(TK, left);
-          if (!(ok = wait1(&bar.empty[r.i], r.par ^ 1, fail))) break;
-          uint8_t* sb = ring + r.i * C::STAGE;
-          uint64_t* full = &bar.full[r.i];
-          uint32_t bytes = 2 * nk * C::KROW;
-          if constexpr (BITS != 0) {
-            // scales and biases: the 16-byte blocks that hold the tile's values
-            const void* const arr[4] = {a.k.scales, a.k.biases, a.v.scales, a.v.biases};
-            uintptr_t src[4];
-            uint32_t len[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uintptr_t p = reinterpret_cast<uintptr_t>(arr[i]) + uintptr_t(i < 2 ? kr : vr) * C::SROW;
-              src[i] = p & ~uintptr_t(15);
-              len[i] = (uint32_t(p & 15) + nk * C::SROW + 15) & ~15u;
-              bytes += len[i];
-            }
-            mbar_arrive_expect_tx(full, bytes);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              bulk_g2s(sb + C::S_OFF + i * C::SWIN, reinterpret_cast<const void*>(src[i]), len[i], full);
-          } else {
-            mbar_arrive_expect_tx(full, bytes);
-          }
-          bulk_g2s(sb + C::K_OFF, reinterpret_cast<const uint8_t*>(a.k.data) + kr * C::KROW, nk * C::KROW, full);
-          bulk_g2s(sb + C::V_OFF, reinterpret_cast<const uint8_t*>(a.v.data) + vr * C::KROW, nk * C::KROW, full);
-          ++issued;
-          r.next();
-        }
+      for (int t = 0; t < w.nt; ++t, from += TK * unit, left -= TK) {
+        const uint32_t skew = lane < 2 ? 0u : uint32_t(reinterpret_cast<uintptr_t>(from)) & 15u;
+        const uint32_t len = lane < COPIES ? (skew + min(TK, left) * unit + 15) & ~15u : 0u;  // rows are multiples of 16
+        const uint32_t bytes = __reduce_add_sync(0xffffffffu, len);
+        if (!(ok = waitw(fail, {&bar.empty[r.i], r.par ^ 1}))) break;
+        if (lane == 0) mbar_arrive_expect_tx(&bar.full[r.i], bytes);
+        __syncwarp();
+        if (lane < COPIES) bulk_g2s(ring + r.i * C::STAGE + to, from - skew, len, &bar.full[r.i]);
+        ++issued;
+        r.next();
       }
-      // the copies in flight land before the CTA may exit: the last min(ST, issued) uses
-      Slot<ST> f;
-#pragma unroll 1
-      for (int i = 0; i < issued; ++i, f.next())
-        if (i >= issued - ST) (void)wait1(&bar.full[f.i], f.par, fail);
     }
+    // the copies in flight land before the CTA may exit: the last min(ST, issued) uses
+    Slot<ST> f;
+#pragma unroll 1
+    for (int i = 0; i < issued; ++i, f.next())
+      if (i >= issued - ST) (void)waitw(fail, {&bar.full[f.i], f.par});
   } else if (warp >= PREP_WARP) {
-    // --------- scales: one warp per stream, or one for tiles both streams take
+    // ---------------------------------------- scales: even tiles, odd tiles
     if constexpr (BITS != 0) {
       Walk w(line, a);
       Slot<ST> r;
       int g = 0;
       bool ok = true;
+      constexpr float SUB = BITS == 8 ? 16777216.f : 1048576.f;  // codes are used as c / SUB
+      using Pair = typename std::conditional<G == 2, uint32_t, uint16_t>::type;  // a key's scales (or biases)
       while (ok && w.next(a, nrb)) {
-        int ev = -127;  // running exponent of V
         const uint32_t kb = uint32_t(w.b * a.k.batch_stride + w.hk * a.k.head_stride);  // only its low bits matter
         const uint32_t vb = uint32_t(w.b * a.v.batch_stride + w.hk * a.v.head_stride);
 #pragma unroll 1
         for (int t = 0; t < w.nt; ++t, ++g, r.next()) {
-          if (TWO ? warp != PREP_WARP : (g & 1) != warp - PREP_WARP) continue;  // V's exponent belongs to a stream
+          if ((g & 1) != warp - PREP_WARP) continue;
           const int key0 = (w.t0 + t) * TK;
           unsigned long long vis = ~0ull;
-          if (key0 + TK > w.n) vis = visible(seen_by_any(a, w.b, lane), key0, w.n, w.kend);
+          const bool edge = key0 + TK > w.n;
+          if (edge) vis = visible(seen_by_any(a, w.b, lane), key0, w.n, w.kend);
           if (!(ok = waitw(fail, {&bar.full[r.i], r.par}))) break;
           uint8_t* sb = ring + r.i * C::STAGE;
-          const void* const arr[4] = {a.k.scales, a.k.biases, a.v.scales, a.v.biases};
-          float s[2][2 * G], b[2][2 * G], mx[2] = {0.f, 0.f};
+          // keys lane and lane + 32: [K, V][key][group]
+          float s[2][2][G], b[2][2][G];
+          uint32_t mx[2];
 #pragma unroll
-          for (int o = 0; o < 2; ++o) {  // K, V
+          for (int o = 0; o < 2; ++o) {
+            const m5_kv_view& view = o ? a.v : a.k;
             const uint32_t at = ((o ? vb : kb) + key0) * C::SROW;
-            const uint8_t* sp = sb + C::S_OFF + 2 * o * C::SWIN + ((uint32_t(reinterpret_cast<uintptr_t>(arr[2 * o])) + at) & 15);
-            const uint8_t* bp = sb + C::S_OFF + (2 * o + 1) * C::SWIN +
-                                ((uint32_t(reinterpret_cast<uintptr_t>(arr[2 * o + 1])) + at) & 15);
+            const uint8_t* sp = sb + C::S_OFF + 2 * o * C::SWIN + ((uint32_t(reinterpret_cast<uintptr_t>(view.scales)) + at) & 15);
+            const uint8_t* bp = sb + C::S_OFF + (2 * o + 1) * C::SWIN + ((uint32_t(reinterpret_cast<uintptr_t>(view.biases)) + at) & 15);
+            float m = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2 * G; ++i) {  // element e of the tile's [64][G]
-              const int e = lane + 32 * i;
-              const bool in = (vis >> (e / G)) & 1;
-              s[o][i] = in ? bf2f(reinterpret_cast<const bf16*>(sp)[e]) : 0.f;
-              b[o][i] = in ? bf2f(reinterpret_cast<const bf16*>(bp)[e]) : 0.f;
-              mx[o] = max3(mx[o], fabsf(b[o][i]), fabsf(fmaf(s[o][i], float((1 << BITS) - 1), b[o][i])));
+            for (int k = 0; k < 2; ++k) {
+              uint32_t sw = reinterpret_cast<const Pair*>(sp)[lane + 32 * k], bw = reinterpret_cast<const Pair*>(bp)[lane + 32 * k];
+              if (edge && !((vis >> (lane + 32 * k)) & 1)) sw = bw = 0;
+#pragma unroll
+              for (int q = 0; q < G; ++q) {
+                s[o][k][q] = q ? bf16_hi(sw) : bf16_lo(sw);
+                b[o][k][q] = q ? bf16_hi(bw) : bf16_lo(bw);
+                m = max3(m, fabsf(b[o][k][q]), fabsf(fmaf(s[o][k][q], float((1 << BITS) - 1), b[o][k][q])));
+              }
             }
-            mx[o] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[o])));
+            mx[o] = __float_as_uint(m);
           }
-          const int ek = top_exp(mx[0], TOPQ);
-          const int e2 = ev = max(ev, top_exp(mx[1], TOPQ));
+          mx[0] = __reduce_max_sync(0xffffffffu, mx[0]);
+          mx[1] = __reduce_max_sync(0xffffffffu, mx[1]);
+          const int ek = top_exp(__uint_as_float(mx[0]), TOPQ);
+          int ev = top_exp(__uint_as_float(mx[1]), TOPQ);
+          // V's exponent runs on within a stream: the tile before it (TWO: settled by the other warp)
+          if (t >= (TWO ? 1 : 2)) {
+            if constexpr (TWO) {
+              static_assert(ST > 2, "the other warp is at most one tile ahead: the stage before is not in use again");
+              const int pi = r.i ? r.i - 1 : ST - 1;
+              if (!(ok = waitw(fail, {&bar.prep[pi], r.i ? r.par : r.par ^ 1}))) break;
+            }
+            ev = max(ev, s_ev[(g - (TWO ? 1 : 2)) & (EXPS - 1)]);
+          }
           if (lane == 0) {
             s_kmul[g & (EXPS - 1)] = pow2(ek);
-            s_ev[g & (EXPS - 1)] = e2;
+            s_ev[g & (EXPS - 1)] = ev;
           }
 #pragma unroll
           for (int o = 0; o < 2; ++o) {
-            const float f = pow2(-(o ? e2 : ek));
-            uint2* dst = reinterpret_cast<uint2*>(sb + C::H_OFF + o * TK * G * 8);
+            const float f = pow2(-(o ? ev : ek)), fs = f * SUB;
+            uint8_t* dst = sb + C::H_OFF + o * TK * G * 8;
 #pragma unroll
-            for (int i = 0; i < 2 * G; ++i) {
-              const float sf = s[o][i] * (f * (BITS == 8 ? 16777216.f : 1048576.f)), bfv = b[o][i] * f;
-              dst[lane + 32 * i] = make_uint2(h2(sf, sf), h2(bfv, bfv));
+            for (int k = 0; k < 2; ++k) {
+              uint32_t v[2 * G];
+#pragma unroll
+              for (int q = 0; q < G; ++q) {
+                const float x = s[o][k][q] * fs, y = b[o][k][q] * f;
+                v[2 * q] = h2(x, x);
+                v[2 * q + 1] = h2(y, y);
+              }
+              if constexpr (G == 2) reinterpret_cast<uint4*>(dst)[lane + 32 * k] = make_uint4(v[0], v[1], v[2], v[3]);
+              else reinterpret_cast<uint2*>(dst)[lane + 32 * k] = make_uint2(v[0], v[1]);
             }
           }
           __syncwarp();
@@ -697,7 +710,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     // write 8 different (chunk ^ key & 7): with two groups they hold the pieces 0-3 of
     // one key and 4-7 of its neighbour (8/4-bit rows), or all pieces of
     // one key with the halves of 4-7 in the other order (bf16 rows of 256 bytes).
-    setmaxnreg_dec<DQ_REGS>();
+    setmaxnreg_dec<C::DQ_REGS>();
     const int o = warp >= SMX_WARPS + DQ_WARPS;  // K, V
     // Packed caches: two warps convert the even tiles of an operand and two the odd ones (a tile's
     // chain of waits, loads, stores and fence is latency, which two tiles at once hide).
@@ -809,7 +822,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     }
   } else if (warp < SMX_WARPS) {
     // ---------------------------------------------------------------- softmax
-    setmaxnreg_inc<SMX_REGS>();
+    setmaxnreg_inc<C::SMX_REGS>();
     const int j = warp >> 3, h = (warp >> 2) & 1, r = tid & 127;  // stream, half of the keys, lane of tensor memory
     const uint32_t lrow = uint32_t(32 * (warp & 3)) << 16;
     constexpr int QPARTS = TWO ? 2 : 4;           // warps that share a row: of its stream, of both

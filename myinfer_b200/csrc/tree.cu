@@ -215,6 +215,10 @@ int m5::tree_attn_check(const TreeAttnArgs& a) {
                "m5_tree_attention: more than 2^31 tiles of 128 rows and 64 keys");
   M5_CHECK_ARG((reinterpret_cast<uintptr_t>(a.k.data) | reinterpret_cast<uintptr_t>(a.v.data)) % 16 == 0,
                "m5_tree_attention: K/V rows must be 16-byte aligned");
+  M5_CHECK_ARG(!a.bits || (reinterpret_cast<uintptr_t>(a.k.scales) | reinterpret_cast<uintptr_t>(a.k.biases) |
+                           reinterpret_cast<uintptr_t>(a.v.scales) | reinterpret_cast<uintptr_t>(a.v.biases)) %
+                                  (a.D / 32) == 0,
+               "m5_tree_attention: a row's scales and biases must be aligned to their size");
   M5_CHECK_ARG((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) % 16 == 0 &&
                    (a.q_sb | a.q_sh | a.q_sl | a.o_sb | a.o_sh | a.o_sl) % 8 == 0,
                "m5_tree_attention: query and output rows must be 16-byte aligned");
