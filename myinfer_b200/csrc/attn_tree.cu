@@ -66,7 +66,6 @@ constexpr float LAZY = 8.f; // log2 growth of a row's maximum that is left in p
 // exact operand without a conversion; scale * 2^24 stays finite when the tile's values,
 // hence 255 scales, stay below 2^-1.
 constexpr int TOP16 = 7, TOPQ = -3;
-constexpr int MIN_TILES = 2;  // per CTA: one per stream
 
 // TWO: a CTA holds two blocks of 128 rows, one per softmax stream; else one
 template <int BITS, int D, bool TWO>
@@ -217,8 +216,21 @@ __device__ __forceinline__ int seq_end(const TreeAttnArgs& a, int n) { return ::
 __device__ __forceinline__ int seq_tiles(const TreeAttnArgs& a, int b) {
   return (seq_end(a, seq_len(a, b)) + TK - 1) / TK;
 }
-__device__ __forceinline__ int part_of(int total, int ctas, int c) { return (int)((long long)total * c / ctas); }
-__device__ __forceinline__ int parts(int total, int ctas) { return ::min(ctas, ::max(1, total / MIN_TILES)); }
+// first tile of part c of `ctas`: floor(total * c / ctas), without a 64-bit division
+__device__ __forceinline__ int part_of(int total, int ctas, int c) {
+  const int q = total / ctas;
+  return c * q + c * (total - q * ctas) / ctas;
+}
+// the part that holds tile t, from a rounded guess
+__device__ __forceinline__ int part_with(int total, int ctas, int t) {
+  int c = ::min(ctas - 1, (int)((float)t * (float)ctas / (float)total));
+  while (part_of(total, ctas, c) > t) --c;
+  while (c + 1 < ctas && part_of(total, ctas, c + 1) <= t) ++c;
+  return c;
+}
+// parts of the line: down to one tile each (a CTA's second tile costs more than a part to join: one
+// node over 512 keys 17.0 us with at least two tiles, 13.9 with one)
+__device__ __forceinline__ int parts(int total, int ctas) { return ::min(ctas, total); }
 // by one warp: this CTA's part of the line
 __device__ __forceinline__ Line part_of_line(const TreeAttnArgs& a, int pairs, int lane, int c, int ctas) {
   Line l{0, 0, a.B - 1, 0, 0};
@@ -997,17 +1009,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
 
 // Joins the partial states of the rows whose run was cut or that were repeated:
 //   o = sum_i w_i O_i / sum_i w_i l_i,  w_i = 2^(m_i - max).
-// One CTA per block of 128 lanes and 16 dims; a thread takes one lane of
-// every second part (the parts of a run are consecutive CTAs), so all loads run
-// along the lanes.  The repeats of a row and the two halves meet in shared memory.
-constexpr int JOIN_DIMS = 16;
-__global__ void __launch_bounds__(2 * ROWS) tree_join_kernel(const TreeAttnArgs a, const int nrb, const int blocks,
-                                                             const int ctas, const float4* part_o,
-                                                             const float2* part_ml) {
-  __shared__ float s_m[2][ROWS], s_l[2][ROWS], s_o[2][ROWS][JOIN_DIMS + 1];
+// One CTA per block of 128 lanes and 8 dims; a thread takes one lane of every
+// fourth part (the parts of a run are consecutive CTAs), so all loads run along
+// the lanes and a run of 40 parts is three rounds of loads.  The repeats of a row and
+// the four quarters of its parts meet in shared memory.
+constexpr int JOIN_DIMS = 8, JOIN_WAYS = 4;
+__global__ void __launch_bounds__(JOIN_WAYS * ROWS) tree_join_kernel(const TreeAttnArgs a, const int nrb, const int blocks,
+                                                                     const int ctas, const float4* part_o,
+                                                                     const float2* part_ml) {
+  __shared__ float s_m[JOIN_WAYS][ROWS], s_l[JOIN_WAYS][ROWS], s_o[JOIN_WAYS][ROWS][JOIN_DIMS + 1];
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, r = tid & (ROWS - 1), half = tid / ROWS;
+  const int tid = threadIdx.x, lane = tid & 31, r = tid & (ROWS - 1), way = tid / ROWS;
   const int grp = a.Hq / a.Hkv, R = a.L * grp, pairs = a.Hkv * nrb;
   int x = blockIdx.x;
   const int blk = x % blocks;
@@ -1026,8 +1039,7 @@ __global__ void __launch_bounds__(2 * ROWS) tree_join_kernel(const TreeAttnArgs 
   base = __reduce_add_sync(0xffffffffu, base);
   const int tiles = seq_tiles(a, b), np = parts(total, ctas);
   const int t0 = base + p * tiles, t1 = t0 + tiles - 1;
-  // part c holds tile t: total * c / np <= t
-  const int c0 = (int)(((t0 + 1LL) * np - 1) / total), c1 = (int)(((t1 + 1LL) * np - 1) / total);
+  const int c0 = part_with(total, np, t0), c1 = part_with(total, np, t1);
   if (c0 == c1 && rep == 1) return;  // written by the attention kernel
   const int n = c1 - c0 + 1, d4 = blockIdx.y * (JOIN_DIMS / 4), D4 = a.D / 4;
   const size_t slot0 = size_t(c0 + b * pairs + p) * blocks + blk;
@@ -1040,9 +1052,9 @@ __global__ void __launch_bounds__(2 * ROWS) tree_join_kernel(const TreeAttnArgs 
   for (int k = 0; k < JOIN_DIMS / 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   if (mine) {
 #pragma unroll 4
-    for (int i = half; i < n; i += 2) m = fmaxf(m, ml[size_t(i) * blocks * ROWS].x);
-#pragma unroll 2
-    for (int i = half; i < n; i += 2) {
+    for (int i = way; i < n; i += JOIN_WAYS) m = fmaxf(m, ml[size_t(i) * blocks * ROWS].x);
+#pragma unroll 4
+    for (int i = way; i < n; i += JOIN_WAYS) {
       const float2 e = ml[size_t(i) * blocks * ROWS];
       const float w = e.x == -INFINITY ? 0.f : ex2(e.x - m);
       l = fmaf(w, e.y, l);
@@ -1056,40 +1068,38 @@ __global__ void __launch_bounds__(2 * ROWS) tree_join_kernel(const TreeAttnArgs 
       }
     }
   }
-  s_m[half][r] = m;
-  s_l[half][r] = l;
+  s_m[way][r] = m;
+  s_l[way][r] = l;
 #pragma unroll
   for (int k = 0; k < JOIN_DIMS / 4; ++k) {
-    s_o[half][r][4 * k] = o[k].x;
-    s_o[half][r][4 * k + 1] = o[k].y;
-    s_o[half][r][4 * k + 2] = o[k].z;
-    s_o[half][r][4 * k + 3] = o[k].w;
+    s_o[way][r][4 * k] = o[k].x;
+    s_o[way][r][4 * k + 1] = o[k].y;
+    s_o[way][r][4 * k + 2] = o[k].z;
+    s_o[way][r][4 * k + 3] = o[k].w;
   }
   __syncthreads();
-  // two threads per row, 8 dims each
-  const int lr = tid >> 1, dh = (tid & 1) * (JOIN_DIMS / 2);
-  if (lr >= nrows) return;
+  if (tid >= nrows) return;  // a thread per row from here on
   float M = -INFINITY;
-  for (int i = 0; i < 2 * rep; ++i) M = fmaxf(M, s_m[i & 1][lr + (i >> 1) * per]);
-  float den = 0.f, num[JOIN_DIMS / 2];
+  for (int i = 0; i < JOIN_WAYS * rep; ++i) M = fmaxf(M, s_m[i % JOIN_WAYS][tid + i / JOIN_WAYS * per]);
+  float den = 0.f, num[JOIN_DIMS];
 #pragma unroll
-  for (int k = 0; k < JOIN_DIMS / 2; ++k) num[k] = 0.f;
-  for (int i = 0; i < 2 * rep; ++i) {
-    const int q = lr + (i >> 1) * per;
-    const float w = s_m[i & 1][q] == -INFINITY ? 0.f : ex2(s_m[i & 1][q] - M);
-    den = fmaf(w, s_l[i & 1][q], den);
+  for (int k = 0; k < JOIN_DIMS; ++k) num[k] = 0.f;
+  for (int i = 0; i < JOIN_WAYS * rep; ++i) {
+    const int y = i % JOIN_WAYS, q = tid + i / JOIN_WAYS * per;
+    const float w = s_m[y][q] == -INFINITY ? 0.f : ex2(s_m[y][q] - M);
+    den = fmaf(w, s_l[y][q], den);
 #pragma unroll
-    for (int k = 0; k < JOIN_DIMS / 2; ++k) num[k] = fmaf(w, s_o[i & 1][q][dh + k], num[k]);
+    for (int k = 0; k < JOIN_DIMS; ++k) num[k] = fmaf(w, s_o[y][q][k], num[k]);
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;
-  const int row = row0 + lr, qi = row / grp, h = p / nrb * grp + row % grp;
+  const int row = row0 + tid, qi = row / grp, h = p / nrb * grp + row % grp;
   uint32_t v[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const __nv_bfloat162 z = __floats2bfloat162_rn(num[2 * k] * inv, num[2 * k + 1] * inv);
     v[k] = *reinterpret_cast<const uint32_t*>(&z);
   }
-  *reinterpret_cast<uint4*>(a.out + b * a.o_sb + h * a.o_sh + qi * a.o_sl + 4 * d4 + dh) = make_uint4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<uint4*>(a.out + b * a.o_sb + h * a.o_sh + qi * a.o_sl + 4 * d4) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 // Launch that may begin while the kernel before it on the stream ends (both
@@ -1131,7 +1141,7 @@ static cudaError_t launch(const TreeAttnArgs& a, const Plan& p, cudaStream_t st)
   float2* ml = reinterpret_cast<float2*>(po + p.slots * ROWS * (D / 4));
   if ((e = launch_early(tree_attn_kernel<BITS, D, TWO>, dim3(p.ctas), dim3(THREADS), C::SMEM, st, a, p.nrb, po, ml)))
     return e;
-  return launch_early(tree_join_kernel, dim3(a.B * a.Hkv * p.nrb * p.blocks, D / JOIN_DIMS), dim3(2 * ROWS), 0, st, a,
+  return launch_early(tree_join_kernel, dim3(a.B * a.Hkv * p.nrb * p.blocks, D / JOIN_DIMS), dim3(JOIN_WAYS * ROWS), 0, st, a,
                       p.nrb, p.blocks, p.ctas, po, ml);
 }
 template <int BITS, int D>
