@@ -99,7 +99,11 @@ def _kv_parts(t: _Kv, bits: int, D: int, dev: int, what: str):
         raise ValueError(f"{what} must be {dtype} [batch, kv heads, rows, {width}] on cuda:{dev}")
     sb, sh, sr, one = data.stride()
     if one != 1 or sr != width or sh % width or sb % width:
-        raise ValueError(f"{what}: a head's rows must be contiguous")
+        # a dimension of size 1 may have any stride: it is never stepped over
+        nb, nh, nr, nw = shape
+        sb, sh = (0 if nb == 1 else sb), (0 if nh == 1 else sh)
+        if (one != 1 and nw > 1) or (sr != width and nr > 1) or sh % width or sb % width:
+            raise ValueError(f"{what}: a head's rows must be contiguous")
     rows_b, rows_h = sb // width, sh // width
     if not bits:
         return M5KvView(data.data_ptr(), None, None, rows_b, rows_h), shape
@@ -108,7 +112,7 @@ def _kv_parts(t: _Kv, bits: int, D: int, dev: int, what: str):
     for x in (s, b):
         if x.dtype is not torch.bfloat16 or x.shape != want or x.get_device() != dev:
             raise ValueError(f"{what}: scales and biases must be bf16 [batch, kv heads, rows, {G}] on cuda:{dev}")
-        if x.stride() != lay:
+        if x.stride() != lay and any(n > 1 and a != b for n, a, b in zip(want, x.stride(), lay)):
             raise ValueError(f"{what}: scales and biases must be laid out like the rows")
     return M5KvView(data.data_ptr(), s.data_ptr(), b.data_ptr(), rows_b, rows_h), shape
 
@@ -153,7 +157,7 @@ def tree_attention(queries: torch.Tensor, q_keys: _Kv, q_values: _Kv, lengths: t
             q = q.clone()
         sb, sh, sl, one = q.stride()
     if out is None:
-        out = torch.empty((B, Hq, L, D), dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != queries.shape or out.dtype is not torch.bfloat16 or out.get_device() != dev or out.stride(3) != 1:
         raise ValueError("out must be bf16 of the queries' shape with contiguous dims")
     need = _workspace_bytes(dev, B, Hq, Hkv, L, D)
@@ -200,7 +204,7 @@ def process_logits(logits: torch.Tensor, batch: Optional[int] = None, counts: Op
     if logits.stride(1) != 1:
         raise ValueError("logits rows must be contiguous")
     if out is None:
-        out = torch.empty((R, V), dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or out.stride(1) != 1:
         raise ValueError("out must have the logits' shape and type, with contiguous rows")
     if (counts is not None or tokens is not None) and penalties is None:
@@ -247,8 +251,9 @@ def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, picks: torch.Tensor
             raise ValueError("counts must be int32 [batch, vocab]")
         V = counts.shape[1]
         cp = _whole(counts, (B, V), "counts", dev)
-    path = torch.empty((B, T), dtype=torch.int32, device=parents.device)
-    n, nxt = torch.empty((2, B), dtype=torch.int32, device=parents.device).unbind(0)
+    path = torch.empty_like(parents)
+    n = parents.new_empty(B)
+    nxt = torch.empty_like(n)
     _launch("m5_tree_accept", dev, parents.data_ptr(), tp, pp, B, T, path.data_ptr(), n.data_ptr(), nxt.data_ptr(), cp, V, V)
     return path, n, nxt
 

@@ -253,6 +253,22 @@ def test_attention_capacity_and_odd_heads():
             _check(_attend(q, k, v, [n], words, D ** -0.5, L, bits), q, k, v, [n], words, D ** -0.5, L, bits)
 
 
+def test_attention_strides_of_single_dimensions():
+    """A dimension of size 1 may have any stride: batch, kv heads and rows of one."""
+    from myinfer_b200.tree import tree_attention
+    rng = np.random.default_rng(12)
+    for bits in (0, 4, 8):
+        for rows in (1, 70):
+            k, v = _cache(rng, 1, 1, rows, 64, bits), _cache(rng, 1, 1, rows, 64, bits)
+            odd = lambda t: t.as_strided(t.shape, (7, 5, 3 if rows == 1 else t.shape[3], 1))  # noqa: E731
+            cut = lambda t: tuple(odd(x.cuda()) for x in t) if bits else odd(t.cuda())  # noqa: E731
+            q = _bf(rng.standard_normal((1, 3, 1, 64))).cuda()
+            n = torch.tensor([rows - 1], dtype=torch.int32).cuda()
+            anc = torch.ones(1, 1, dtype=torch.int64).cuda()
+            out = tree_attention(q, cut(k), cut(v), n, anc, 0.125, bits=bits)
+            _check(out, q, k, v, [rows - 1], np.ones((1, 1), np.uint64), 0.125, 1, bits)
+
+
 def test_attention_far_offsets():
     """A head that starts more than 2^31 bytes and 2^30 elements into the cache."""
     from myinfer_b200.tree import tree_attention
