@@ -35,9 +35,6 @@
 // value.  Q is scaled per row in the same way, which is exact.  Scores, maxima,
 // sums and O are fp32.  A row's maximum is only moved when a new score exceeds
 // it by 2^8 (p <= 256 in fp16): O is rescaled rarely.
-// With 64 rows or fewer, the idle lanes repeat the rows and take a part of each
-// tile's keys (64 rows: halves, 32: quarters), which divides the exponentials of a
-// warp by 2 or 4; their states are joined like those of other CTAs.
 // TMEM columns: S / P [stream][2] 64 each, O [stream] 128 each.
 #include <algorithm>
 #include <cmath>
@@ -301,9 +298,6 @@ struct Walk {
   __device__ __forceinline__ bool whole() const { return nt == tiles; }
 };
 
-// Rows of a block (nrows of 128) repeat 4, 2 or 1 times over the lanes.
-__device__ __forceinline__ int repeats(int nrows) { return nrows <= 32 ? 4 : nrows <= 64 ? 2 : 1; }
-
 // Tree keys that some query of sequence b sees (by one warp).
 __device__ __forceinline__ unsigned long long seen_by_any(const TreeAttnArgs& a, int b, int lane) {
   unsigned long long w = 0;
@@ -341,11 +335,6 @@ __device__ __forceinline__ uint4 conv16(uint4 w, float f) {
                     h2(bf16_lo(w.z) * f, bf16_hi(w.z) * f), h2(bf16_lo(w.w) * f, bf16_hi(w.w) * f));
 }
 
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
 
 // O *= f over D dims of this thread's row.
 template <int D>
@@ -382,12 +371,11 @@ struct Row {
 // columns of those keys.  pair: barrier of the two warps that share the
 // rows (0: this warp has them alone), mine / other: where they exchange maxima.
 // Returns the factor by which O has to change.
-template <int N>
 __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, float c, bool edge,
                                               unsigned long long vis, int pair, float* mine, const float* other) {
+  constexpr int N = TK / 2;
   float s[N];
-  if constexpr (N == 32) tmem_ld32(s_addr + off, s);
-  else tmem_ld16(s_addr + off, s);
+  tmem_ld32(s_addr + off, s);
   tmem_ld_wait();
   if (edge) {
     const uint32_t v = uint32_t(vis >> off);
@@ -405,12 +393,10 @@ __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, 
   float mt = tmax == -INFINITY ? -INFINITY : tmax * c, corr = 1.f;
   const bool up = mt > r.m + LAZY;  // also: the first score the row sees (r.m = -inf)
   // both warps have read their S here, so either's P may overwrite it
-  if (pair ? pair_or(pair, up) : __any_sync(0xffffffffu, up)) {
-    if (pair) {
-      *mine = mt;
-      named_sync(pair, 64);
-      mt = fmaxf(mt, *other);
-    }
+  if (pair_or(pair, up)) {
+    *mine = mt;
+    named_sync(pair, 64);
+    mt = fmaxf(mt, *other);
     if (mt > r.m + LAZY) {
       corr = r.m == -INFINITY ? 0.f : ex2(r.m - mt);
       r.m = mt;
@@ -428,8 +414,7 @@ __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, 
     p[i / 2] = h2(e.x, e.y);
   }
   r.l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-  if constexpr (N == 32) tmem_st16(s_addr + off / 2, p);
-  else tmem_st8(s_addr + off / 2, p);
+  tmem_st16(s_addr + off / 2, p);
   return corr;
 }
 
@@ -845,14 +830,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
     bool ok = true;
     while (ok && w.next(a, nrb)) {
       const int row0 = (w.rb * C::BLOCKS + (TWO ? j : 0)) * ROWS, nrows = max(0, min(ROWS, R - row0));
-      const int rep = repeats(nrows), per = ROWS / rep;
-      const int lr = r % per, rr = r / per;         // row of the block, its repeat
-      const bool row_ok = lr < nrows;
-      const int row = row_ok ? row0 + lr : 0, qi = row / grp, hq = w.hk * grp + row % grp;
-      // keys of this warp: 32 h (one repeat), 32 rr + 16 h (two), 16 rr (four: half 0 alone)
-      const int off = rep == 1 ? 32 * h : rep == 2 ? 32 * rr + 16 * h : 16 * rr;
-      const bool idle = lr - lane >= nrows || (rep == 4 && h);  // nothing to do for the whole warp (per is a multiple of 32)
-      const int pair = rep == 4 || lr - lane >= nrows ? 0 : pair_id;
+      const bool row_ok = r < nrows, idle = r - lane >= nrows;  // idle: the whole warp has no row
+      const int row = row_ok ? row0 + r : 0, qi = row / grp, hq = w.hk * grp + row % grp;
       const unsigned long long word = a.anc[w.b * a.anc_sb + qi];
       // Q, scaled by a power of two per row; the sign of `scale` goes with it
       float c_row;
@@ -901,20 +880,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
           const unsigned long long vis = edge ? visible(word, key0, w.n, w.kend) : 0ull;
           const float c = c_row * s_kmul[g & (EXPS - 1)];
           const uint32_t sa = tmem + lrow + S_COL + 64u * buf;
-          float corr;
-          if (rep == 1) {
-            corr = softmax_tile<32>(st, sa, off, c, edge, vis, pair, &s_xl[j][h][r], &s_xl[j][h ^ 1][r]);
-          } else {
-            corr = softmax_tile<16>(st, sa, off, c, edge, vis, pair, &s_xl[j][h][r], &s_xl[j][h ^ 1][r]);
-            // P of the keys other repeats take is zero: half of them, or (one warp) all
-            const uint32_t z[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-            if (rep == 2) {
-              tmem_st8(sa + 16u * (rr ^ 1) + 8u * h, z);
-            } else {
-#pragma unroll
-              for (int k = 1; k < 4; ++k) tmem_st8(sa + 8u * ((rr + k) & 3), z);
-            }
-          }
+          float corr = softmax_tile(st, sa, 32 * h, c, edge, vis, pair_id, &s_xl[j][h][r], &s_xl[j][h ^ 1][r]);
           // V's exponent in this stream; for bf16 caches it is there once the tile's V is (whose
           // buffer cannot be refilled before this P is used: its phase stands still)
           if (BITS == 0) ok = ok && waitw(fail, {&bar.vfull[g % NOP], uint32_t(g / NOP) & 1});
@@ -924,9 +890,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             if (__any_sync(0xffffffffu, corr != 1.f)) {  // the same for both warps: each takes half of the dims
               ok = ok && waitw(fail, {&bar.pvdone[buf ^ 1], uint32_t((u - 1) >> 1) & 1});
               tc_fence_after();
-              const uint32_t oa = tmem + lrow + O_COL + 128u * j;
-              if (pair) scale_o<D / 2>(oa + h * (D / 2), corr);
-              else scale_o<D>(oa, corr);
+              scale_o<D / 2>(tmem + lrow + O_COL + 128u * j + h * (D / 2), corr);
             }
           }
           st.ev = ev;
@@ -948,14 +912,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
       named_sync(1, SMX_WARPS * 32);
       tc_fence_after();
       if (tid == 0) s_stop = *fail;
-      if (ok && lr - lane < nrows) {
+      if (ok && r - lane < nrows) {
         // the two streams' states of the row, joined; TWO: the stream's own
         const int j0 = TWO ? j : 0;
         const float mx = s_m[j0][r], my = TWO ? -INFINITY : s_m[1][r], M = fmaxf(mx, my);
         const float wx = mx == -INFINITY ? 0.f : ex2(mx - M), wy = my == -INFINITY ? 0.f : ex2(my - M);
         float l = (s_xl[j0][0][r] + s_xl[j0][1][r]) * wx;
         if constexpr (!TWO) l += (s_xl[1][0][r] + s_xl[1][1][r]) * wy;
-        const bool direct = w.whole() && rep == 1;
+        const bool direct = w.whole();
         const float inv = direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
         const float fx = wx * pow2(s_oev[j0][r]) * inv, fy = TWO ? 0.f : wy * pow2(s_oev[1][r]) * inv;
         const size_t slot = size_t(blockIdx.x + w.pair) * C::BLOCKS + (TWO ? j : 0);
@@ -1007,12 +971,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
   }
 }
 
-// Joins the partial states of the rows whose run was cut or that were repeated:
+// Joins the partial states of the rows whose run was cut:
 //   o = sum_i w_i O_i / sum_i w_i l_i,  w_i = 2^(m_i - max).
-// One CTA per block of 128 lanes and 8 dims; a thread takes one lane of every
+// One CTA per block of 128 rows and 8 dims; a thread takes one row of every
 // fourth part (the parts of a run are consecutive CTAs), so all loads run along
-// the lanes and a run of 40 parts is three rounds of loads.  The repeats of a row and
-// the four quarters of its parts meet in shared memory.
+// the rows and a run of 40 parts is three rounds of loads (the idle lanes of 32 rows or
+// fewer as 16 ways: no faster).  The four quarters of a row's parts meet in shared memory.
 constexpr int JOIN_DIMS = 8, JOIN_WAYS = 4;
 __global__ void __launch_bounds__(JOIN_WAYS * ROWS) tree_join_kernel(const TreeAttnArgs a, const int nrb, const int blocks,
                                                                      const int ctas, const float4* part_o,
@@ -1028,7 +992,6 @@ __global__ void __launch_bounds__(JOIN_WAYS * ROWS) tree_join_kernel(const TreeA
   const int p = x % pairs, b = x / pairs;
   const int row0 = (p % nrb * blocks + blk) * ROWS, nrows = min(ROWS, R - row0);
   if (nrows <= 0) return;
-  const int rep = repeats(nrows), per = ROWS / rep;
   int total = 0, base = 0;  // tiles of all sequences, and of those before b
   for (int i = lane; i < a.B; i += 32) {
     const int t = seq_tiles(a, i) * pairs;
@@ -1040,17 +1003,16 @@ __global__ void __launch_bounds__(JOIN_WAYS * ROWS) tree_join_kernel(const TreeA
   const int tiles = seq_tiles(a, b), np = parts(total, ctas);
   const int t0 = base + p * tiles, t1 = t0 + tiles - 1;
   const int c0 = part_with(total, np, t0), c1 = part_with(total, np, t1);
-  if (c0 == c1 && rep == 1) return;  // written by the attention kernel
+  if (c0 == c1) return;  // written by the attention kernel
   const int n = c1 - c0 + 1, d4 = blockIdx.y * (JOIN_DIMS / 4), D4 = a.D / 4;
   const size_t slot0 = size_t(c0 + b * pairs + p) * blocks + blk;
-  const bool mine = r % per < nrows;
   const float2* ml = part_ml + slot0 * ROWS + r;
   const float4* po = part_o + (slot0 * D4 + d4) * ROWS + r;
   float m = -INFINITY, l = 0.f;
   float4 o[JOIN_DIMS / 4];
 #pragma unroll
   for (int k = 0; k < JOIN_DIMS / 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (mine) {
+  if (r < nrows) {
 #pragma unroll 4
     for (int i = way; i < n; i += JOIN_WAYS) m = fmaxf(m, ml[size_t(i) * blocks * ROWS].x);
 #pragma unroll 4
@@ -1080,16 +1042,17 @@ __global__ void __launch_bounds__(JOIN_WAYS * ROWS) tree_join_kernel(const TreeA
   __syncthreads();
   if (tid >= nrows) return;  // a thread per row from here on
   float M = -INFINITY;
-  for (int i = 0; i < JOIN_WAYS * rep; ++i) M = fmaxf(M, s_m[i % JOIN_WAYS][tid + i / JOIN_WAYS * per]);
+#pragma unroll
+  for (int y = 0; y < JOIN_WAYS; ++y) M = fmaxf(M, s_m[y][tid]);
   float den = 0.f, num[JOIN_DIMS];
 #pragma unroll
   for (int k = 0; k < JOIN_DIMS; ++k) num[k] = 0.f;
-  for (int i = 0; i < JOIN_WAYS * rep; ++i) {
-    const int y = i % JOIN_WAYS, q = tid + i / JOIN_WAYS * per;
-    const float w = s_m[y][q] == -INFINITY ? 0.f : ex2(s_m[y][q] - M);
-    den = fmaf(w, s_l[y][q], den);
 #pragma unroll
-    for (int k = 0; k < JOIN_DIMS; ++k) num[k] = fmaf(w, s_o[y][q][k], num[k]);
+  for (int y = 0; y < JOIN_WAYS; ++y) {
+    const float w = s_m[y][tid] == -INFINITY ? 0.f : ex2(s_m[y][tid] - M);
+    den = fmaf(w, s_l[y][tid], den);
+#pragma unroll
+    for (int k = 0; k < JOIN_DIMS; ++k) num[k] = fmaf(w, s_o[y][tid][k], num[k]);
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;
   const int row = row0 + tid, qi = row / grp, h = p / nrb * grp + row % grp;
