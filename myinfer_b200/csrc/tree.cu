@@ -94,9 +94,11 @@ struct CommitTable {
 };
 
 constexpr int kCommitThreads = 128;
-constexpr int kCommitUnits = kTreeMax * 256 / 16 / kCommitThreads;  // 16-byte units per thread of the widest rows (bf16, D = 128)
 
-__global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __grid_constant__ CommitTable t, int Hkv,
+// UNITS: 16-byte units per thread of 64 of the widest rows (256 bytes: 8).  The registers they take
+// decide how many of the small CTAs an SM holds (4 requests x 64 layers are 4096).
+template <int UNITS>
+__global__ void __launch_bounds__(kCommitThreads, UNITS == 2 ? 16 : UNITS == 4 ? 10 : 7) tree_commit_kernel(const __grid_constant__ CommitTable t, int Hkv,
                                                                      const int32_t* lengths, const int32_t* path,
                                                                      int T, const int32_t* accepted) {
   __shared__ int s_path[kTreeMax];
@@ -114,9 +116,9 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __gri
   const size_t base = size_t(blockIdx.x) * ly.capacity + len;
   uint4* data = reinterpret_cast<uint4*>(ly.p[kv]);
   const int per = ly.row / 16;  // 16-byte units of a row: 2 to 16, a power of two
-  uint4 u[kCommitUnits];
+  uint4 u[UNITS];
 #pragma unroll
-  for (int k = 0; k < kCommitUnits; ++k) {
+  for (int k = 0; k < UNITS; ++k) {
     const int e = tid + k * kCommitThreads, r = e / per;
     if (r < n && s_path[r] >= 0) u[k] = data[(base + s_path[r]) * per + e % per];
   }
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const __gri
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kCommitUnits; ++k) {
+  for (int k = 0; k < UNITS; ++k) {
     const int e = tid + k * kCommitThreads, r = e / per;
     if (r < n && s_path[r] >= 0) data[(base + r) * per + e % per] = u[k];
   }
@@ -184,6 +186,7 @@ extern "C" int m5_tree_commit(const m5_layer_kv* layers, int num_layers, int B, 
   }
   for (int l0 = 0; l0 < num_layers; l0 += kTreeLayers) {
     CommitTable t;
+    int row = 0;  // widest
     const int nl = std::min(kTreeLayers, num_layers - l0);
     for (int i = 0; i < nl; ++i) {
       const m5_layer_kv& l = layers[l0 + i];
@@ -192,9 +195,10 @@ extern "C" int m5_tree_commit(const m5_layer_kv* layers, int num_layers, int B, 
       t.layer[i].capacity = l.capacity;
       t.layer[i].row = l.bits ? D * l.bits / 8 : 2 * D;
       t.layer[i].group = l.bits ? D / 64 * 2 : 0;
+      row = std::max(row, t.layer[i].row);
     }
-    tree_commit_kernel<<<dim3(B * Hkv, nl, 2), kCommitThreads, 0, (cudaStream_t)stream>>>(t, Hkv, lengths, path, T,
-                                                                                         accepted);
+    const auto kernel = row <= 64 ? tree_commit_kernel<2> : row <= 128 ? tree_commit_kernel<4> : tree_commit_kernel<8>;
+    kernel<<<dim3(B * Hkv, nl, 2), kCommitThreads, 0, (cudaStream_t)stream>>>(t, Hkv, lengths, path, T, accepted);
     M5_LAUNCH_CHECK("tree commit launch");
   }
   return M5_OK;
