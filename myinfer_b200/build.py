@@ -4,6 +4,8 @@ Usage: ``python -m myinfer_b200.build [--verbose]``.  Every ``csrc/*.cu`` is
 compiled for ``sm_100a`` only (``-gencode arch=compute_100a,code=sm_100a``),
 without fast-math (the KV quantizer must round exactly like the CPU rule),
 and linked into ``myinfer_b200/libm5cuda.so`` next to this file.
+``csrc/tree_binding.cpp`` (the Python entries of the tree operators, against torch's
+headers) becomes ``myinfer_b200/_tree_binding.so``.
 """
 
 from __future__ import annotations
@@ -13,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -20,6 +23,7 @@ CSRC = HERE / "csrc"
 OBJ = HERE / "_build"
 LIB = HERE / "libm5cuda.so"
 INCLUDE = HERE.parent / "include"
+BINDING = HERE / "_tree_binding.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -63,8 +67,28 @@ def _compile(src: Path, verbose: bool) -> Path:
     return out
 
 
+def build_binding() -> Path:
+    import torch
+
+    src, root = CSRC / "tree_binding.cpp", Path(torch.__file__).resolve().parent
+    deps = [src, INCLUDE / "m5cuda.h", root / "version.py"]
+    if BINDING.exists() and all(BINDING.stat().st_mtime >= d.stat().st_mtime for d in deps):
+        return BINDING
+    # nvcc's host compiler, as for libm5cuda: another one ($CXX) may bring a C++ library of its own into the process
+    cmd = [nvcc(), "-O2", "-std=c++17", "-shared", "--cudart", "none", "-Xcompiler", "-fPIC,-fvisibility=hidden", str(src), "-o",
+           str(BINDING), f"-I{INCLUDE}", f"-I{sysconfig.get_paths()['include']}", "-isystem", str(root / "include"),
+           "-isystem", str(root / "include/torch/csrc/api/include"),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-L{root / 'lib'}", "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_python", "-Xlinker", f"-rpath={root / 'lib'}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{src.name}:\n{r.stderr}")
+    return BINDING
+
+
 def build(verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
+    build_binding()
     srcs = sorted(CSRC.glob("*.cu"))
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
