@@ -14,9 +14,13 @@
 //               rows of one (layer, K or V, head) go through registers of one
 //               CTA, loads before stores, so sources and destinations may
 //               overlap in any way.  All layers are one launch: the table of
-//               their buffers travels as the kernel's parameter.
-// None of them moves enough bytes to matter (a commit of 20 rows over 64 layers is
-// 5 MB): they are bound by launch and by one or two dependent trips to memory.
+//               their buffers travels as the kernel's parameter (of 32, 64 or 128
+//               layers: 8 KB of it cost the host 0.5 us more than 2).
+// None of them moves enough bytes to matter (a commit of 20 rows over 64 layers
+// is 5 MB): they are bound by their launch and by one to three dependent trips to
+// memory.  Accepting, one tree of 8 or 64 trees of 64 nodes: 2.0 us on the device.  A
+// commit of 28 layers, 8 heads, 8 bits: 3.2 us; of 64 layers for 4 requests, 4 bits: 5.9 us
+// (11 MB, 1.9 TB/s).
 #include <algorithm>
 
 #include "tree.cuh"
@@ -84,21 +88,22 @@ __global__ void __launch_bounds__(kTreeMax) tree_accept_kernel(const int32_t* pa
   }
 }
 
+template <int LAYERS>
 struct CommitTable {
   struct {
     void* p[6];        // K data, scales, biases, V data, scales, biases
     int64_t capacity;
     int32_t row;       // bytes of a data row
     int32_t group;     // bytes of a scale row (0: bf16 cache)
-  } layer[kTreeLayers];
+  } layer[LAYERS];
 };
 
 constexpr int kCommitThreads = 128;
 
 // UNITS: 16-byte units per thread of 64 of the widest rows (256 bytes: 8).  The registers they take
 // decide how many of the small CTAs an SM holds (4 requests x 64 layers are 4096).
-template <int UNITS>
-__global__ void __launch_bounds__(kCommitThreads, UNITS == 2 ? 16 : UNITS == 4 ? 10 : 7) tree_commit_kernel(const __grid_constant__ CommitTable t, int Hkv,
+template <int UNITS, int LAYERS>
+__global__ void __launch_bounds__(kCommitThreads, UNITS == 2 ? 16 : UNITS == 4 ? 10 : 7) tree_commit_kernel(const __grid_constant__ CommitTable<LAYERS> t, int Hkv,
                                                                      const int32_t* lengths, const int32_t* path,
                                                                      int T, const int32_t* accepted) {
   __shared__ int s_path[kTreeMax];
@@ -140,6 +145,29 @@ __global__ void __launch_bounds__(kCommitThreads, UNITS == 2 ? 16 : UNITS == 4 ?
 #pragma unroll
     for (int k = 0; k < 2; ++k) reinterpret_cast<uint16_t*>(ly.p[kv + 1 + k])[(base + sr) * gr + tid % gr] = s[k];
   }
+}
+
+// One launch for the first layers (as many as the table holds).
+template <int LAYERS>
+int commit_some(const m5_layer_kv* layers, int left, int B, int Hkv, int D, const int32_t* lengths, const int32_t* path,
+                int T, const int32_t* accepted, void* stream) {
+  CommitTable<LAYERS> t;
+  int row = 0;  // widest
+  const int nl = std::min(LAYERS, left);
+  for (int i = 0; i < nl; ++i) {
+    const m5_layer_kv& l = layers[i];
+    void* const p[6] = {l.k, l.k_scales, l.k_biases, l.v, l.v_scales, l.v_biases};
+    std::copy(p, p + 6, t.layer[i].p);
+    t.layer[i].capacity = l.capacity;
+    t.layer[i].row = l.bits ? D * l.bits / 8 : 2 * D;
+    t.layer[i].group = l.bits ? D / 64 * 2 : 0;
+    row = std::max(row, t.layer[i].row);
+  }
+  const auto kernel = row <= 64 ? tree_commit_kernel<2, LAYERS> : row <= 128 ? tree_commit_kernel<4, LAYERS>
+                                                                             : tree_commit_kernel<8, LAYERS>;
+  kernel<<<dim3(B * Hkv, nl, 2), kCommitThreads, 0, (cudaStream_t)stream>>>(t, Hkv, lengths, path, T, accepted);
+  M5_LAUNCH_CHECK("tree commit launch");
+  return M5_OK;
 }
 
 }  // namespace
@@ -184,22 +212,11 @@ extern "C" int m5_tree_commit(const m5_layer_kv* layers, int num_layers, int B, 
     M5_CHECK_ARG((reinterpret_cast<uintptr_t>(l.k) | reinterpret_cast<uintptr_t>(l.v)) % 16 == 0,
                  "m5_tree_commit: K/V rows must be 16-byte aligned");
   }
-  for (int l0 = 0; l0 < num_layers; l0 += kTreeLayers) {
-    CommitTable t;
-    int row = 0;  // widest
-    const int nl = std::min(kTreeLayers, num_layers - l0);
-    for (int i = 0; i < nl; ++i) {
-      const m5_layer_kv& l = layers[l0 + i];
-      void* const p[6] = {l.k, l.k_scales, l.k_biases, l.v, l.v_scales, l.v_biases};
-      std::copy(p, p + 6, t.layer[i].p);
-      t.layer[i].capacity = l.capacity;
-      t.layer[i].row = l.bits ? D * l.bits / 8 : 2 * D;
-      t.layer[i].group = l.bits ? D / 64 * 2 : 0;
-      row = std::max(row, t.layer[i].row);
-    }
-    const auto kernel = row <= 64 ? tree_commit_kernel<2> : row <= 128 ? tree_commit_kernel<4> : tree_commit_kernel<8>;
-    kernel<<<dim3(B * Hkv, nl, 2), kCommitThreads, 0, (cudaStream_t)stream>>>(t, Hkv, lengths, path, T, accepted);
-    M5_LAUNCH_CHECK("tree commit launch");
+  for (int l0 = 0; l0 < num_layers;) {
+    const int left = num_layers - l0;
+    const auto some = left <= 32 ? commit_some<32> : left <= 64 ? commit_some<64> : commit_some<kTreeLayers>;
+    if (int rc = some(layers + l0, left, B, Hkv, D, lengths, path, T, accepted, stream)) return rc;
+    l0 += kTreeLayers;
   }
   return M5_OK;
 }
