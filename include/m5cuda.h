@@ -286,7 +286,8 @@ M5_API int m5_tree_attention_workspace(int B, int Hq, int Hkv, int L, int D, siz
  * step of sequences of different lengths), Hq a multiple of Hkv, D 64 or 128,
  * bits 8/4 (groups of 64) or 0 (bf16).  q, out: bf16 with strides {batch,
  * head, query} in elements (multiples of 8) and contiguous dims; keys, values:
- * `capacity` rows per head, rows 16-byte aligned.  Keys at or above capacity
+ * `capacity` rows per head, rows 16-byte aligned, a row's scales and biases
+ * aligned to their size (D / 32 bytes).  Keys at or above capacity
  * do not exist.  Rows no query sees are not used, whatever they hold.  Scores,
  * maxima and sums are fp32; nothing is rounded to bf16 before the output.
  * workspace: 16-byte aligned, not shared by calls that may overlap. */

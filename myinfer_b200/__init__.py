@@ -9,7 +9,9 @@ carry device memory and streams.  Modules:
 * ``attention``     blocked_quantized_sdpa / safe_maybe_quantize_kv_cache
 * ``cache``         device KVCache / QuantizedKVCache / make_prompt_cache
 * ``model``         Qwen3 / Qwen3-MoE model handle, random-init weights
-* ``generate``      chunked prefill + CUDA-graph greedy decode loop
+* ``tree``          operators of speculation over a tree of drafted tokens
+* ``generate``      chunked prefill + CUDA-graph decode loop, speculation over a
+                    chain or a tree of drafts
 * ``context``, ``prefix_cache``, ``engine``  the reference's host policy
 """
 

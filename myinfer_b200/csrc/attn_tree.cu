@@ -35,7 +35,19 @@
 // value.  Q is scaled per row in the same way, which is exact.  Scores, maxima,
 // sums and O are fp32.  A row's maximum is only moved when a new score exceeds
 // it by 2^8 (p <= 256 in fp16): O is rescaled rarely.
-// TMEM columns: S / P [stream][2] 64 each, O [stream] 128 each.
+// TMEM columns: S / P [stream][2] 64 each, O [stream] 128 each (all 512).
+//
+// Time on the device (launches in a graph, inputs of 3 sets in turn): 2 rows a kv head over
+// 512 keys 12.8 us (two launches, one tile per CTA and a join: latency); 128 rows x 8 kv heads over
+// 131072 keys, 4 bits: 105 us = 654 TFLOP/s, 1.44 TB/s; 512 rows x 8 kv heads over 32768 keys, 8
+// bits: 97 us = 710 TFLOP/s.  Long calls are bound by the chain of hand-overs of a tile (a
+// poll of a complete barrier takes 80-190 cycles, commit to wait 230) together with the issue
+// slots: at 512 rows 61 % of the slots, tensor cores 57 % of the cycles at the 1.64 GHz the
+// power limit leaves, DRAM 10 %; a copy without any arithmetic in conversion and softmax still
+// took 64-70 us.  What did not pay: 8 softmax warps (110 us at 512 rows), one lane polling for its warp
+// (166), S and PV from two warps (113), one thread as MMA warp with its waits polled ahead (104),
+// 128 keys per hand-over (104: a stream's next S then waits for its PV), few rows repeated over
+// the idle lanes of a tile (103; one node over 512 keys 13.7).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -1088,6 +1100,10 @@ struct Plan {
 };
 static Plan plan(int B, int Hq, int Hkv, int L) {
   const long long rows = (long long)L * (Hq / Hkv);
+  // Two blocks of rows per converted tile (one: two parts convert each tile) from 129 rows on, over
+  // 32768 keys: 256 rows 58.8 us (one: 62.9), 512 rows 95.0 (112.7), bf16 122.5 (176.7); 128 rows
+  // 49.1 (one: 42.7), the second stream idle.  Over 600 keys one would do: 256 rows 19.0 (16.1), 512
+  // 25.8 (26.0); the lengths are not known here.
   const int blocks = rows > ROWS ? 2 : 1, nrb = ceil_div(rows, ROWS * blocks), ctas = sm_count();
   return {nrb, blocks, ctas, (size_t(ctas) + size_t(B) * Hkv * nrb) * blocks};
 }

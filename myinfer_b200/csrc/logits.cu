@@ -20,6 +20,11 @@
 // of a token is the one that counts, and it (else the token's last path entry)
 // is the one that writes, so no order of threads matters.  The row's choice is a
 // maximum over (value, lowest index) words, joined over the cluster in shared memory.
+//
+// On the device: one bf16 row of 151936 with penalties 5.8 us (latency: loads, cluster join);
+// a tree of 64 such rows with 300 biases and masks 28.2 us (40.7 MB from and to memory, 1.44 TB/s;
+// the counts, read again for every row from L2, take 7 us of it, the biases 6.5, the masks 2.5,
+// a plain copy 10); 40 fp32 rows of 32001, unaligned, 13.3 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -15,6 +15,10 @@ the next token back (the argmax, or the device sampler's draw, which also
 applies the logits processors and rolls their token window on the device), so
 the host only copies 4 bytes per token out.
 
+With a draft model the loop verifies a chain of its tokens per model call, or
+with ``tree_widths`` a tree of them (``tree_speculative_generate_step``), under
+whole-context penalties, token biases and a grammar's bit masks.
+
 Every kernel wait is bounded: a wait that runs out (a copy that never landed,
 a peer rank that never arrived) records a device error word instead of
 hanging.  The loop reads those words after the prompt, every
