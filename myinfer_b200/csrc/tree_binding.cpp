@@ -3,11 +3,11 @@
 //
 // A small call's kernels take 2 us (accepting a path) to 13 us (attention over a
 // short cache), so what the host does before them is the call's time: accepting
-// took 13.0 us a call with ctypes and takes 6.8, a commit of 28 layers 11.0 and 7.0, one
-// row of logits 12.7 and 8.2, attention over 512 keys 22.2 and 13.1 (its kernels).  The kernels
-// and the C ABI are libm5cuda.so's,
-// whose addresses `bind` receives; errors are ValueError for what a tensor must be,
-// and the library's status through the `check` it receives too.
+// took 13.0 us a call with ctypes and takes 6.8, a commit of 28 layers 11.0 and 6.9,
+// one row of logits 12.7 and 8.2, attention over 512 keys 22.2 and 13.1 (its kernels).
+// The kernels and the C ABI are libm5cuda.so's, whose addresses `bind` receives.  Errors
+// are ValueError for what a tensor must be, and the library's status through the
+// `check` that `bind` receives too.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
