@@ -79,7 +79,7 @@ def build_binding() -> Path:
            str(BINDING), f"-I{INCLUDE}", f"-I{sysconfig.get_paths()['include']}", "-isystem", str(root / "include"),
            "-isystem", str(root / "include/torch/csrc/api/include"),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-L{root / 'lib'}", "-lc10", "-lc10_cuda",
-           "-ltorch_cpu", "-ltorch_python", "-Xlinker", f"-rpath={root / 'lib'}"]
+           "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Xlinker", f"-rpath={root / 'lib'}"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{src.name}:\n{r.stderr}")

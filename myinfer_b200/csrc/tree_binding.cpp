@@ -3,12 +3,13 @@
 //
 // A small call's kernels take 2 us (accepting a path) to 13 us (attention over a
 // short cache), so what the host does before them is the call's time: accepting
-// took 13.0 us a call with ctypes and takes 6.8, a commit of 28 layers 11.0 and 6.9,
+// took 13.0 us a call with ctypes and takes 6.5, a commit of 28 layers 11.0 and 7.5,
 // one row of logits 12.7 and 8.2, attention over 512 keys 22.2 and 13.1 (its kernels).
 // The kernels and the C ABI are libm5cuda.so's, whose addresses `bind` receives.  Errors
 // are ValueError for what a tensor must be, and the library's status through the
 // `check` that `bind` receives too.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -82,6 +83,11 @@ void expect(Py_ssize_t got, Py_ssize_t want) {
   TORCH_CHECK_TYPE(got == want, "expected ", want, " arguments, got ", got);
 }
 
+// An uninitialised tensor on a device, past the operator dispatch (0.3 us of a call each).
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, int dev) {
+  return at::detail::empty_cuda(shape, type, c10::Device(c10::DeviceType::CUDA, static_cast<c10::DeviceIndex>(dev)), std::nullopt);
+}
+
 const at::Tensor& trees(PyObject* o) {
   const at::Tensor& t = tensor(o, "parents");
   TORCH_CHECK_VALUE(t.dim() == 2 && t.scalar_type() == at::kInt && t.is_cuda() && t.is_contiguous(),
@@ -134,7 +140,7 @@ PyObject* plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
   expect(n, 1);
   const at::Tensor& parents = trees(args[0]);
   const int B = small(parents.size(0)), T = small(parents.size(1)), dev = parents.get_device();
-  at::Tensor anc = at::empty({B, T}, parents.options().dtype(at::kLong)), depth = at::empty({B, T}, parents.options());
+  at::Tensor anc = empty({B, T}, at::kLong, dev), depth = empty({B, T}, at::kInt, dev);
   if (!launch(dev, [&](void* st) {
         return fn.plan((const int32_t*)parents.data_ptr(), B, T, (int64_t*)anc.data_ptr(), (int32_t*)depth.data_ptr(), st);
       }))
@@ -224,7 +230,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   at::Tensor out;
   if (args[9] == Py_None) {
-    out = at::empty({B, Hq, L, D}, q.options());
+    out = empty({B, Hq, L, D}, at::kBFloat16, dev);
   } else {
     out = tensor(args[9], "out");
     TORCH_CHECK_VALUE(out.dim() == 4 && out.scalar_type() == at::kBFloat16 && out.sizes() == q.sizes() && out.is_cuda() &&
@@ -236,7 +242,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!launch(dev, [&](void* st) {
         size_t need = 0;
         if (int rc = fn.workspace(small(B), small(Hq), small(Hkv), small(L), small(D), &need)) return rc;
-        ws = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+        ws = empty({(int64_t)need}, at::kByte, dev);
         return fn.attention(q.data_ptr(), qs.s, small(B), small(Hq), small(L), small(D), k, v, small(Hkv), rows, lengths,
                             small(T), anc, L, (float)scale, (int)group, (int)bits, out.data_ptr(), os.s, ws.data_ptr(), need, st);
       }))
@@ -262,7 +268,7 @@ PyObject* logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   TORCH_CHECK_VALUE(x.stride(1) == 1 || V == 1, "logits rows must be contiguous");
   at::Tensor out;
   if (args[9] == Py_None) {
-    out = at::empty({R, V}, x.options());
+    out = empty({R, V}, x.scalar_type(), dev);
   } else {
     out = tensor(args[9], "out");
     TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && out.device() == x.device() &&
@@ -291,7 +297,7 @@ PyObject* logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     mld = last(args[8], "mask");
     mp = whole(args[8], {R, mld}, "mask", dev);
   }
-  at::Tensor choices = at::empty({R}, x.options().dtype(at::kInt));
+  at::Tensor choices = empty({R}, at::kInt, dev);
   // a single row's stride is meaningless (torch keeps any stride on a size-1 dimension)
   const int64_t ld = R > 1 ? x.stride(0) : V, old = R > 1 ? out.stride(0) : V;
   const int dt = x.scalar_type() == at::kBFloat16 ? M5_DTYPE_BF16 : M5_DTYPE_F32;
@@ -322,8 +328,8 @@ PyObject* accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
     V = counts.size(1);
     cp = (int32_t*)whole(args[3], {B, V}, "counts", dev);
   }
-  at::Tensor path = at::empty({B, T}, parents.options()), count = at::empty({B}, parents.options()),
-             next = at::empty({B}, parents.options());
+  at::Tensor path = empty({B, T}, at::kInt, dev), count = empty({B}, at::kInt, dev),
+             next = empty({B}, at::kInt, dev);
   if (!launch(dev, [&](void* st) {
         return fn.accept((const int32_t*)parents.data_ptr(), tp, pp, small(B), small(T), (int32_t*)path.data_ptr(),
                          (int32_t*)count.data_ptr(), (int32_t*)next.data_ptr(), cp, V, V, st);

@@ -152,7 +152,8 @@ class CacheLayers:
         self.batch, self.kv_heads, self.head_dim = shape
         if self.head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {self.head_dim}")
-        self.structs, self.address = arr, ctypes.addressof(arr)
+        self.structs = arr
+        self.call = (ctypes.addressof(arr), len(arr), self.batch, self.kv_heads, self.head_dim, self.device.index)
 
 
 def commit_tree(layers, lengths: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
@@ -161,4 +162,4 @@ def commit_tree(layers, lengths: torch.Tensor, path: torch.Tensor, accepted: tor
     place.  ``layers``: a ``CacheLayers`` (a loop keeps one), or what it takes.
     ``lengths`` is left to the caller to advance."""
     t = layers if isinstance(layers, CacheLayers) else CacheLayers(layers)
-    (_calls or _load()).commit(t.address, len(t.structs), t.batch, t.kv_heads, t.head_dim, t.device.index, lengths, path, accepted)
+    (_calls or _load()).commit(*t.call, lengths, path, accepted)
