@@ -109,6 +109,10 @@ __device__ __forceinline__ unsigned long long lp_key(float v, int w) {
   return ((unsigned long long)u << 32) | (0xFFFFFFFFu - (uint32_t)w);
 }
 
+// All CTAs of a cluster have arrived before any thread passes the wait (nothing is ordered by it).
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // 8 entries of a thread: raw bits of consecutive ones (VEC), or of entries 32 apart.
 template <typename T, bool VEC>
 struct Group {
@@ -260,6 +264,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) process_logits_kernel(const Log
   __shared__ int s_n;
   const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.y, b = r / a.T, t = r - b * a.T;
   const int v0 = blockIdx.x * a.per, v1 = min(a.V, v0 + a.per);
+  if (a.choices) cluster_arrive();  // this CTA has started: the others' join may write to its shared memory
   const T* in = reinterpret_cast<const T*>(a.in) + r * a.in_ld;
   T* out = reinterpret_cast<T*>(a.out) + r * a.out_ld;
   const int32_t* counts = a.counts ? a.counts + b * a.counts_ld : nullptr;
@@ -356,6 +361,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) process_logits_kernel(const Log
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if ((tid & 31) == 0) s_best[tid >> 5] = best;
   __syncthreads();
+  cluster_wait();  // rank 0 has started (a part with nothing to do gets here before it)
   cg::cluster_group cl = cg::this_cluster();
   if (tid == 0) {
     for (int i = 1; i < kLpThreads / 32; ++i) best = max(best, s_best[i]);

@@ -440,6 +440,33 @@ def test_process_logits_strides_nan_and_ties():
     assert c.item() == 100 and one.shape == (1, V)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_process_logits_parts_without_work(dtype):
+    """The choice is joined over a row's CTAs, whichever starts or ends first: all but one part masked out (their CTAs
+    load nothing), rows of one part, and calls close behind one another on two streams."""
+    from myinfer_b200.tree import process_logits
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for R, V in ((1, 65536), (1, 65541), (3, 4097), (40, 12000)):
+        x = torch.randn(R, V, generator=g, device="cuda").to(dtype)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        masks, want = [], []
+        for part in range(16):
+            lo, hi = part * V // 16, (part + 1) * V // 16
+            keep = torch.zeros(R, (V + 31) // 32 * 32, dtype=torch.int64, device="cuda")
+            keep[:, lo:hi] = 1
+            m = (keep.view(R, -1, 32) << torch.arange(32, device="cuda")).sum(-1)
+            masks.append(m.to(torch.uint32).view(torch.int32))
+            want.append(lo + x[:, lo:hi].float().argmax(1).to(torch.int32))
+        torch.cuda.synchronize()
+        got = []
+        for i in range(64):
+            with torch.cuda.stream(streams[i & 1]):
+                got.append(process_logits(x, mask=masks[i % 16])[1])
+        torch.cuda.synchronize()
+        for i, c in enumerate(got):
+            assert torch.equal(c, want[i % 16]), (R, V, i)
+
+
 def test_process_logits_matches_greedy_sampler_without_processors():
     from myinfer_b200 import ops
     from myinfer_b200.tree import process_logits
