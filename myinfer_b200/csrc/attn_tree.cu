@@ -426,6 +426,7 @@ __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, 
     p[i / 2] = h2(e.x, e.y);
   }
   r.l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+  __syncwarp();  // lanes whose maximum moved and those whose did not: the store is the whole warp's
   tmem_st16(s_addr + off / 2, p);
   return corr;
 }
@@ -860,6 +861,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
                                      __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
         // the largest exponent of the whole row
         s_qmax[2 * j + h][r] = mx;
+        __syncwarp();
         named_sync(1, SMX_WARPS * 32);
 #pragma unroll
         for (int i = 0; i < QPARTS; ++i) mx = __vmaxu2(mx, s_qmax[TWO ? 2 * j + i : i][r]);
@@ -924,6 +926,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
       named_sync(1, SMX_WARPS * 32);
       tc_fence_after();
       if (tid == 0) s_stop = *fail;
+      __syncwarp();  // the loads of tensor memory below are the whole warp's
       if (ok && r - lane < nrows) {
         // the two streams' states of the row, joined; TWO: the stream's own
         const int j0 = TWO ? j : 0;
@@ -948,8 +951,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             const int dim = BITS == 4 ? (k & 8) + ((k & 7) >> 1) + 4 * (k & 1) : k;
             o[dim] = (wx > 0.f ? o0[k] * fx : 0.f) + (!TWO && wy > 0.f ? o1[k] * fy : 0.f);
           }
-          if (!row_ok) continue;
-          if (direct) {
+          if (row_ok && direct) {
             uint4 v[2];
             uint32_t* p = reinterpret_cast<uint32_t*>(v);
 #pragma unroll
@@ -959,14 +961,16 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
             }
             reinterpret_cast<uint4*>(out + d0)[0] = v[0];
             reinterpret_cast<uint4*>(out + d0)[1] = v[1];
-          } else {
+          } else if (row_ok) {
             float4* po = part_o + (slot * (D / 4) + d0 / 4) * ROWS + r;  // [slot][dim / 4][row]: rows side by side
 #pragma unroll
             for (int k = 0; k < 4; ++k) po[k * ROWS] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
+          __syncwarp();  // lanes without a row meet the others before the next load
         }
         if (!direct && row_ok && qp == 0) part_ml[slot * ROWS + r] = make_float2(M, l);
       }
+      __syncwarp();
       tc_fence_before();
       named_sync(1, SMX_WARPS * 32);  // O and Q may be overwritten
       tc_fence_after();

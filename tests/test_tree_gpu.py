@@ -160,6 +160,21 @@ def test_attention_long(bits, B, Hq, Hk, L, D, n):
 
 
 @pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("rows", [1, 31, 33, 97, 127, 129, 161, 255])
+def test_attention_rows_of_part_of_a_warp(rows, bits):
+    """A warp's lanes with and without a row load tensor memory together: every count of rows around a warp's 32 and a
+    block's 128, in runs that one CTA ends (few keys) and that are cut into parts."""
+    rng = np.random.default_rng(rows)
+    G = next(g for g in range(1, rows + 1) if rows % g == 0 and rows // g <= 64)  # heads on the one kv head
+    L, D = rows // G, 128
+    words = np.full((1, L), ~np.uint64(0))
+    for n in (0, 1000):
+        q = _bf(rng.standard_normal((1, G, L, D))).cuda()
+        k, v = _cache(rng, 1, 1, n + L, D, bits), _cache(rng, 1, 1, n + L, D, bits)
+        _check(_attend(q, k, v, [n], words, D ** -0.5, L, bits), q, k, v, [n], words, D ** -0.5, L, bits)
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
 def test_attention_masks_and_garbage(bits):
     """Rows that see nothing are zero; rows nobody sees may hold NaN and infinities."""
     rng = np.random.default_rng(5)
