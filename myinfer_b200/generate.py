@@ -431,8 +431,6 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
                 tokens[0, row1:row1 + len(lv) * w] = lg.float().topk(w, dim=-1).indices.reshape(-1).to(torch.int32)
             row0 = row1
         model.forward_tree(tokens[0], mcache, depths[0], ancestors[0], 0, _lib.M5_LOGITS_ALL, logits)
-        for cache in (mcache, dcache):
-            safe_maybe_quantize_kv_cache(cache, quantized_kv_start, kv_group_size, kv_bits)
         mask = None if grammar is None else grammar(seen, tokens[0].tolist(), parents[0].tolist())
         _, picks = process_logits(logits, batch=1, counts=counts, penalties=pen,
                                   tokens=None if pen is None else tokens, ancestors=None if pen is None else ancestors,
@@ -452,6 +450,8 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
         for cache in (mcache, dcache):
             for c in cache:
                 c.offset += k
+            # only here: a conversion keeps the committed rows alone, none of a tree that is not committed yet
+            safe_maybe_quantize_kv_cache(cache, quantized_kv_start, kv_group_size, kv_bits)
         _lib.device_check()
         seen += kept
         for t in kept[1:]:

@@ -281,7 +281,8 @@ class Model:
         ancestor words [L] as ``tree.tree_plan`` makes them) behind the cache's
         committed rows: node i goes to row ``cache.offset + row0 + i``.  The
         offset stays; accept a path with ``tree.tree_accept`` and
-        ``tree.commit_tree``, then add its length to every layer's offset."""
+        ``tree.commit_tree``, then add its length to every layer's offset.
+        Until then the rows are none of the cache's own: quantizing it drops them."""
         L = int(tokens.numel())
         for t, dt, what in ((tokens, torch.int32, "tokens"), (depths, torch.int32, "depths"),
                             (ancestors, torch.int64, "ancestors")):

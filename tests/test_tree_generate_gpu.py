@@ -186,3 +186,41 @@ def test_stream_generate_tree():
     out = list(stream_generate(main, Tok(), [3, 1, 4, 1, 5], 10, draft_model=draft, tree_widths=(2, 2), kv_bits=8,
                                prefill_step_size=16))
     assert len(out) == 10 and out[-1].finish_reason == "length"
+
+
+def _rows(cache, n):
+    """K and V of the first n rows, fp32 [layers, 2, Hkv, n, D]."""
+    from myinfer_b200 import ops
+    return torch.stack([torch.stack([(ops.dequantize(*t, 64, c.bits) if c.bits else t)[0, :, :n].float()
+                                     for t in (c.keys, c.values)]) for c in cache])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("cached,prompt_len,start", [(0, 30, 40), (0, 1, 0), (20, 1, 0)],
+                         ids=["threshold_crossed", "one_token", "given_bf16_cache"])
+def test_rows_survive_quantization(cached, prompt_len, start, bits):
+    """The cache turns to 8/4 bits while the loop runs: the committed rows are those of a fresh prefill of the same
+    tokens.  Both were rounded to codes, at most a step (a fifteenth of a group's range, 0.3 of a row's
+    size) and what the layers below make of it apart: less than half of a row's size; a lost row is off by all of it."""
+    from myinfer_b200.cache import KVCache, make_prompt_cache
+    from myinfer_b200.generate import tree_speculative_generate_step
+    main, draft = _model(MAIN, 41), _model(DRAFT, 42)
+    rng = np.random.default_rng(prompt_len)
+    before = rng.integers(0, MAIN["vocab_size"], cached).tolist()
+    prompt = rng.integers(0, MAIN["vocab_size"], prompt_len).tolist()
+    caches = []
+    for m in (main, draft):
+        caches.append(_prefilled(m, before, None) if cached else make_prompt_cache(m))
+    n = 20
+    got = list(tree_speculative_generate_step(prompt, main, draft, (2, 2, 1), n, prompt_cache=caches[0],
+                                              draft_cache=caches[1], prefill_step_size=16, kv_bits=bits,
+                                              quantized_kv_start=start))
+    assert len(got) == n
+    ctx = before + prompt + [t for t, _ in got]
+    for m, cache in zip((main, draft), caches):
+        assert not any(type(c) is KVCache for c in cache)
+        rows = min(cache.offset, len(ctx))
+        assert rows >= len(ctx) - 1
+        have, want = _rows(cache, rows), _rows(_prefilled(m, ctx[:rows], bits), rows)
+        err = (have - want).norm(dim=-1) / want.norm(dim=-1)
+        assert err.max().item() < 0.5, (err > 0.5).nonzero()[:5].tolist()
