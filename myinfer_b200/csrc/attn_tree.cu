@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
         for (int i = 0; i < QPARTS; ++i) mx = __vmaxu2(mx, s_qmax[TWO ? 2 * j + i : i][r]);
         const int eq = top_exp(__uint_as_float(max(mx & 0xFFFFu, mx >> 16) << 16), TOP16);
         const float f = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
-        c_row = fmaxf(fabsf(a.scale) * LOG2E * pow2(eq), 1e-37f);
+        c_row = fabsf(a.scale) * LOG2E * pow2(eq);
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
           const int ch = qp * NQ + i;
@@ -892,7 +892,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
           tc_fence_after();
           const bool edge = key0 + TK > w.n;
           const unsigned long long vis = edge ? visible(word, key0, w.n, w.kend) : 0ull;
-          const float c = c_row * s_kmul[g & (EXPS - 1)];
+          // Above 0, for a hidden score is -inf and times 0 NaN: rows and tiles of zeros (exponents of -100 both)
+          // come to 1e-61, and so does a scale of 0.  S is below 2^23 here, times 1e-37 it is nothing.
+          float c = c_row * s_kmul[g & (EXPS - 1)];
+          if (c < 1e-37f) c = 1e-37f;  // (a NaN stays)
           const uint32_t sa = tmem + lrow + S_COL + 64u * buf;
           float corr = softmax_tile(st, sa, 32 * h, c, edge, vis, pair_id, &s_xl[j][h][r], &s_xl[j][h ^ 1][r]);
           // V's exponent in this stream; for bf16 caches it is there once the tile's V is (whose

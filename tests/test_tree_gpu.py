@@ -598,3 +598,24 @@ def test_refusals():
             tree.CacheLayers(bad)
     with pytest.raises(ValueError):
         tree.commit_tree([(k, k)], n, p, n)
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("keys", ["zero", "tiny", "last tile zero", "any"])
+@pytest.mark.parametrize("n,T", [(0, 1), (5, 2), (64, 5), (70, 3), (1024, 7), (1000, 64)])
+def test_attention_zero_queries_and_keys(n, T, keys, bits):
+    """A query of zeros weighs all keys alike, and so do keys of zeros: in tiles with hidden keys, in tiles that hide
+    all of theirs (tree keys that the row does not see, behind a whole tile), in runs that are cut."""
+    rng = np.random.default_rng(n + T)
+    for D, Hq in ((64, 2), (128, 20)):
+        q = 1.5 * rng.standard_normal((1, Hq, T, D))
+        q[:, ::2] = 0
+        q[:, 1, 0] = 1e-36
+        x = rng.standard_normal((1, 1, n + T, D)).astype(np.float32)
+        x *= dict(zero=0.0, tiny=1e-36).get(keys, 1.0)
+        if keys == "last tile zero":
+            x[:, :, n // 64 * 64:] = 0
+        q, k = _bf(q).cuda(), (_pack(x, bits) if bits else _bf(x))
+        v = _cache(rng, 1, 1, n + T, D, bits)
+        for words in (ref.ancestors(_trees(rng, 1, T))[0], np.zeros((1, T), np.uint64)):
+            _check(_attend(q, k, v, [n], words, D ** -0.5, T, bits), q, k, v, [n], words, D ** -0.5, T, bits)
