@@ -328,6 +328,11 @@ __device__ __forceinline__ unsigned long long visible(unsigned long long word, i
   return (word << -rel) | ((1ull << -rel) - 1);
 }
 
+// Does a query with this word see any key?
+__device__ __forceinline__ bool sees_any(unsigned long long word, int n, int kend) {
+  return n > 0 || visible(word, n, n, kend) != 0;
+}
+
 // fp16 (K, V): 8 consecutive dims of a row into one 16-byte chunk.
 // 8-bit: byte c is the fp16 subnormal c * 2^-24; s (times 2^24) and b are exact
 // (bf16 values), so code * s + b is rounded once.  An offset of the code folded into b
@@ -938,7 +943,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
         float l = (s_xl[j0][0][r] + s_xl[j0][1][r]) * wx;
         if constexpr (!TWO) l += (s_xl[1][0][r] + s_xl[1][1][r]) * wy;
         const bool direct = w.whole();
+        // no weight: the row sees no key (0), or its scores are all -inf (0 / 0)
+        if (direct && l == 0.f && sees_any(a.anc[w.b * a.anc_sb + qi], w.n, w.kend)) l = NAN;
         const float inv = direct ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+        // a stream without a finite score has no O to add, but its NaN counts
+        const bool ux = wx > 0.f || l != l, uy = !TWO && (wy > 0.f || l != l);
         const float fx = wx * pow2(s_oev[j0][r]) * inv, fy = TWO ? 0.f : wy * pow2(s_oev[1][r]) * inv;
         const size_t slot = size_t(blockIdx.x + w.pair) * C::BLOCKS + (TWO ? j : 0);
         bf16* out = a.out + w.b * a.o_sb + hq * a.o_sh + qi * a.o_sl;
@@ -952,7 +961,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             const int dim = BITS == 4 ? (k & 8) + ((k & 7) >> 1) + 4 * (k & 1) : k;
-            o[dim] = (wx > 0.f ? o0[k] * fx : 0.f) + (!TWO && wy > 0.f ? o1[k] * fy : 0.f);
+            o[dim] = (ux ? o0[k] * fx : 0.f) + (uy ? o1[k] * fy : 0.f);
           }
           if (row_ok && direct) {
             uint4 v[2];
@@ -992,6 +1001,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attn_kernel(const TreeAttnArg
 
 // Joins the partial states of the rows whose run was cut:
 //   o = sum_i w_i O_i / sum_i w_i l_i,  w_i = 2^(m_i - max).
+// A part without a finite score has m = -inf and counts for nothing, but for a sum of NaN.
 // One CTA per block of 128 rows and 8 dims; a thread takes one row of every
 // fourth part (the parts of a run are consecutive CTAs), so all loads run along
 // the rows and a run of 40 parts is three rounds of loads (the idle lanes of 32 rows or
@@ -1073,8 +1083,12 @@ __global__ void __launch_bounds__(JOIN_WAYS * ROWS) tree_join_kernel(const TreeA
 #pragma unroll
     for (int k = 0; k < JOIN_DIMS; ++k) num[k] = fmaf(w, s_o[y][tid][k], num[k]);
   }
-  const float inv = den == 0.f ? 0.f : 1.f / den;
   const int row = row0 + tid, qi = row / grp, h = p / nrb * grp + row % grp;
+  float inv = 1.f / den;
+  if (den == 0.f) {  // as at the end of a run that was not cut
+    const int sn = seq_len(a, b);
+    inv = sees_any(a.anc[b * a.anc_sb + qi], sn, seq_end(a, sn)) ? NAN : 0.f;
+  }
   uint32_t v[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {

@@ -619,3 +619,41 @@ def test_attention_zero_queries_and_keys(n, T, keys, bits):
         v = _cache(rng, 1, 1, n + T, D, bits)
         for words in (ref.ancestors(_trees(rng, 1, T))[0], np.zeros((1, T), np.uint64)):
             _check(_attend(q, k, v, [n], words, D ** -0.5, T, bits), q, k, v, [n], words, D ** -0.5, T, bits)
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("n", [0, 40, 3000])
+@pytest.mark.parametrize("T", [4, 40])
+def test_attention_queries_without_a_number(T, n, bits):
+    """What the softmax makes no number of is NaN, in runs that one CTA ends and in runs that are cut: a query with NaN
+    or an infinity, scores that are all -inf, a scale of NaN.  A query that sees nothing gives zeros whatever it
+    holds, and the other queries of the call what they give without it."""
+    rng = np.random.default_rng(T)
+    D, Hq = 128, 4
+    q = _bf(rng.standard_normal((1, Hq, T, D)))
+    k, v = _cache(rng, 1, 1, n + T, D, bits), _cache(rng, 1, 1, n + T, D, bits)
+    words = np.array([[(1 << (i + 1)) - 1 for i in range(T)]], np.uint64)  # a chain
+    clean = _attend(q.cuda(), k, v, [n], words, 0.1, T, bits)
+    bad = q.clone()
+    bad[0, 0, 1, 3] = math.nan
+    bad[0, 1, 1, 5] = math.inf
+    bad[0, 2, 3] = math.nan
+    out = _attend(bad.cuda(), k, v, [n], words, 0.1, T, bits)
+    rows = torch.zeros(1, Hq, T, dtype=torch.bool)
+    rows[0, 0, 1] = rows[0, 1, 1] = rows[0, 2, 3] = True
+    assert torch.isnan(out[rows]).all() and torch.equal(out[~rows], clean[~rows])
+    assert torch.isnan(_attend(q.cuda(), k, v, [n], words, math.nan, T, bits)).all()
+    k0 = k.clone() if bits == 0 else tuple(t.clone() for t in k)
+    if bits:
+        k0[1].fill_(0.0)
+        k0[2].fill_(2.0)   # every key is 2 in all dims
+    else:
+        k0.fill_(2.0)
+    low = q.clone()
+    low[0, 3, 2, 7] = -math.inf
+    out = _attend(low.cuda(), k0, v, [n], words, 0.1, T, bits)
+    assert torch.isnan(out[0, 3, 2]).all() and torch.isfinite(out[0, :3]).all()
+    if n == 0:
+        words[0, 1] = words[0, 2] = 0
+        for x, kk in ((bad, k), (low, k0)):
+            assert (_attend(x.cuda(), kk, v, [n], words, 0.1, T, bits)[0, :, 1:3] == 0).all()
