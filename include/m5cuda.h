@@ -288,8 +288,10 @@ M5_API int m5_tree_attention_workspace(int B, int Hq, int Hkv, int L, int D, siz
  * head, query} in elements (multiples of 8) and contiguous dims; keys, values:
  * `capacity` rows per head, rows 16-byte aligned, a row's scales and biases
  * aligned to their size (D / 32 bytes).  Keys at or above capacity
- * do not exist.  Rows no query sees are not used, whatever they hold.  Scores,
- * maxima and sums are fp32; nothing is rounded to bf16 before the output.
+ * do not exist.  Rows no query sees are not used, whatever they hold; a row with
+ * NaN or an infinity makes NaN or infinities of the queries that see it (the whole
+ * row NaN where it is a tree key's value), and is nothing to the others.
+ * Scores, maxima and sums are fp32; nothing is rounded to bf16 before the output.
  * workspace: 16-byte aligned, not shared by calls that may overlap. */
 M5_API int m5_tree_attention(const void* q, const int64_t* q_strides, int B, int Hq, int L, int D, m5_kv_view keys,
                              m5_kv_view values, int Hkv, int64_t capacity, const int32_t* lengths, int tree_len,

@@ -68,7 +68,8 @@ def tree_attention(queries: torch.Tensor, q_keys: _Kv, q_values: _Kv, lengths: t
     ``bits=0``.  lengths: int32 [B] committed keys, seen by every query.
     ancestors: int64 [B, L], bit j = the query sees tree key ``lengths[b] + j``;
     ``tree_len`` (default L) is the number of tree keys.  A query that sees no
-    key gives zeros.  Returns bf16 [B, Hq, L, D] (``out`` if given)."""
+    key gives zeros; a key or value with NaN or an infinity spoils the queries
+    that see it, no others.  Returns bf16 [B, Hq, L, D] (``out`` if given)."""
     return (_calls or _load()).attention(queries, q_keys, q_values, lengths, ancestors, scale, tree_len, group_size, bits, out)
 
 

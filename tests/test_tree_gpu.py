@@ -657,3 +657,63 @@ def test_attention_queries_without_a_number(T, n, bits):
         words[0, 1] = words[0, 2] = 0
         for x, kk in ((bad, k), (low, k0)):
             assert (_attend(x.cuda(), kk, v, [n], words, 0.1, T, bits)[0, :, 1:3] == 0).all()
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads", [1, 20])
+def test_attention_broken_node(heads, bad, bits):
+    """A node whose key or value holds NaN or an infinity spoils the queries that see it and no others: their
+    results are those of a run in which its row is zero, whatever shares the tile, the run or the call with it."""
+    rng = np.random.default_rng(heads)
+    B, Hk, T, D, node = 2, 2, 8, 128, 2
+    for lengths in ([130, 5], [60, 127], [2000, 640]):
+        q = _bf(rng.standard_normal((B, Hk * heads, T, D))).cuda()
+        k, v = (_cache(rng, B, Hk, max(lengths) + T, D, bits) for _ in range(2))
+        words = ref.ancestors(_trees(rng, B, T))[0]
+        sees = torch.zeros(B, T, dtype=torch.bool)
+        sees[0] = torch.from_numpy((words[0] >> np.uint64(node) & np.uint64(1)).astype(bool))
+        assert 0 < sees[0].sum() < T
+        at = (0, slice(None), lengths[0] + node)
+        for which in (0, 1):
+            kv = [tuple(x.clone() for x in t) if bits else t.clone() for t in (k, v)]
+            for x in kv[which] if bits else (kv[which],):
+                x[at] = 0
+            want = _attend(q, *kv, lengths, words, 0.1, T, bits).transpose(1, 2).cpu()
+            for part in (kv[which][1:] if bits else (kv[which],)):   # a group's scale, its bias; one element
+                part[(*at, 1 if bits else 77)] = bad
+                out = _attend(q, *kv, lengths, words, 0.1, T, bits).transpose(1, 2).cpu()
+                assert torch.equal(out[~sees], want[~sees]), (which, lengths)
+                if which or math.isnan(bad):                          # an infinite key may weigh nothing
+                    assert not torch.isfinite(out[sees]).all(-1).any(), (which, lengths)
+                part[(*at, 1 if bits else 77)] = 0
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+def test_attention_broken_committed_key(bits):
+    """All queries see a committed key.  NaN in K gives NaN, NaN in V at least in the elements that hold it; a score of
+    -inf weighs nothing and leaves the other keys' weights as they are."""
+    rng = np.random.default_rng(4)
+    Hk, T, D, n = 2, 3, 128, 700
+    q = _bf(np.abs(rng.standard_normal((1, 4, T, D)))).cuda()
+    k, v = (_cache(rng, 1, Hk, n + T, D, bits) for _ in range(2))
+    words = ref.ancestors(_trees(rng, 1, T))[0]
+
+    def put(t, value, at):
+        t = tuple(x.clone() for x in t) if bits else t.clone()
+        if bits:
+            t[1][0, :, at, 0] = 0.0      # scale 0, bias the value: the whole first group
+            t[2][0, :, at, 0] = value
+        else:
+            t[0, :, at, :64] = value
+        return t
+
+    def without(t, at):
+        cut = lambda x: torch.cat([x[:, :, :at], x[:, :, at + 1:]], 2)  # noqa: E731
+        return tuple(cut(x) for x in t) if bits else cut(t)
+    for at in (10, 64 * 5 + 63, n - 1):
+        assert torch.isnan(_attend(q, put(k, math.nan, at), v, [n], words, 0.05, T, bits)).all()
+        out = _attend(q, k, put(v, math.nan, at), [n], words, 0.05, T, bits)
+        assert torch.isnan(out[..., :64]).all()
+        out = _attend(q, put(k, -math.inf, at), v, [n], words, 0.05, T, bits)
+        _check(out, q, without(k, at), without(v, at), [n - 1], words, 0.05, T, bits)
