@@ -394,6 +394,7 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
     total = mcache.offset + len(prompt) + max_tokens + T
     for m in (model, draft_model):
         m.reserve(max(T, min(prefill_step_size, max(1, len(prompt) - 1))))
+    t0 = time.perf_counter()
     for m, cache in ((model, mcache), (draft_model, dcache)):
         for p0 in range(0, len(prompt) - 1, prefill_step_size):
             m.forward(prompt_t[p0:min(p0 + prefill_step_size, len(prompt) - 1)], cache)
@@ -416,6 +417,8 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
     tables, sig = None, None
     ntoks = 0
     if stats is not None:
+        torch.cuda.current_stream(dev).synchronize()  # the prompt has run: its time ends here
+        stats["prompt_time"] = time.perf_counter() - t0
         stats["prompt_tokens"] = len(prompt)
     t1 = time.perf_counter()
     while ntoks < max_tokens:

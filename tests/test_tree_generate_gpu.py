@@ -224,3 +224,20 @@ def test_rows_survive_quantization(cached, prompt_len, start, bits):
         have, want = _rows(cache, rows), _rows(_prefilled(m, ctx[:rows], bits), rows)
         err = (have - want).norm(dim=-1) / want.norm(dim=-1)
         assert err.max().item() < 0.5, (err > 0.5).nonzero()[:5].tolist()
+
+
+def test_prompt_and_decode_times():
+    """The prompt's rate is of its own time, and the generation's does not hold it."""
+    from myinfer_b200.generate import stream_generate, tree_speculative_generate_step
+
+    class Tok:
+        eos_token_ids = []
+
+        def decode(self, ids):
+            return " ".join(str(i) for i in ids)
+    main, draft = _model(MAIN, 31), _model(DRAFT, 32)
+    stats = {}
+    list(tree_speculative_generate_step(list(range(200)), main, draft, (2,), 4, stats=stats, prefill_step_size=16))
+    assert stats["prompt_tokens"] == 200 and stats["prompt_time"] > 0 and stats["decode_time"] > 0
+    last = list(stream_generate(main, Tok(), list(range(200)), 4, draft_model=draft, tree_widths=(2,), prefill_step_size=16))[-1]
+    assert 0 < last.prompt_tps < 1e7  # 200 tokens in 26 calls of the two models: not in 20 us
