@@ -354,7 +354,8 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
                                    grammar: Optional[Callable] = None, prompt_cache: Optional[PromptCache] = None,
                                    draft_cache: Optional[PromptCache] = None, prefill_step_size: int = 2048,
                                    kv_bits: Optional[int] = None, kv_group_size: int = 64,
-                                   quantized_kv_start: int = 0, stats: Optional[dict] = None) -> Iterator[tuple]:
+                                   quantized_kv_start: int = 0, stats: Optional[dict] = None,
+                                   context_tokens: Optional[List[int]] = None) -> Iterator[tuple]:
     """Speculative decoding over a tree of drafts: each round the draft model
     proposes, for every node of a level, its ``tree_widths[d]`` likeliest tokens,
     the main model scores all nodes in one call, and the longest path whose
@@ -366,10 +367,12 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
 
     ``sampler``: a ``DeviceSampler`` draws the choices from the processed logits
     (its own penalty window is not used).  ``penalties`` = (repetition, presence,
-    frequency) over the whole context; ``logit_bias`` maps token ids to added
+    frequency) over the context: the prompt, what is generated, and ``context_tokens``,
+    the tokens that a given ``prompt_cache`` already holds (all of them, in order; left
+    out, they do not count).  ``logit_bias`` maps token ids to added
     values; ``grammar(tokens, nodes, parents)`` returns the int32 bit mask
     [len(nodes), ceil(V / 32)] on the device for the tokens that may follow each
-    node (``tokens``: everything before the tree, ``nodes``: the nodes' tokens) or None."""
+    node (``tokens``: the context before the tree, ``nodes``: the nodes' tokens) or None."""
     if not prompt:
         raise ValueError("empty prompt")
     V = model.args.vocab_size
@@ -388,6 +391,11 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
     dcache = draft_cache if draft_cache is not None else make_prompt_cache(draft_model)
     if mcache.offset != dcache.offset:
         raise ValueError("the two caches hold different lengths")
+    context = [int(t) for t in context_tokens or []]
+    if context_tokens is not None and len(context) != mcache.offset:
+        raise ValueError(f"context_tokens are {len(context)} tokens, the cache holds {mcache.offset}")
+    if context and (min(context) < 0 or max(context) >= V):
+        raise ValueError(f"context_tokens: token id out of range [0, {V})")
     prompt_t = torch.as_tensor(prompt, dtype=torch.int32).to(dev)
     parents = torch.tensor([[p for lv in levels for p in lv]], dtype=torch.int32).to(dev)
     ancestors, depths = tree_plan(parents)
@@ -401,10 +409,11 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
             safe_maybe_quantize_kv_cache(cache, quantized_kv_start, kv_group_size, kv_bits)
         for c in cache:
             c.reserve(total)
+    seen = context + list(prompt[:-1])
     counts = pen = ids = values = None
     if penalties is not None:
         pen = torch.tensor([list(penalties)], dtype=torch.float32).to(dev)
-        counts = torch.bincount(prompt_t[:-1].long(), minlength=V).to(torch.int32)[None].contiguous()
+        counts = torch.bincount(torch.as_tensor(seen, dtype=torch.int64).to(dev), minlength=V).to(torch.int32)[None]
     if logit_bias:
         ids = torch.tensor([list(logit_bias)], dtype=torch.int32).to(dev)
         values = torch.tensor([list(logit_bias.values())], dtype=torch.float32).to(dev)
@@ -413,7 +422,6 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
     logits = torch.empty(T, V, dtype=torch.bfloat16, device=dev)
     d_logits = torch.empty(max(len(lv) for lv in levels), V, dtype=torch.bfloat16, device=dev)
     lengths = torch.zeros(1, dtype=torch.int32, device=dev)
-    seen = list(prompt[:-1])
     tables, sig = None, None
     ntoks = 0
     if stats is not None:

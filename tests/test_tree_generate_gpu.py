@@ -241,3 +241,30 @@ def test_prompt_and_decode_times():
     assert stats["prompt_tokens"] == 200 and stats["prompt_time"] > 0 and stats["decode_time"] > 0
     last = list(stream_generate(main, Tok(), list(range(200)), 4, draft_model=draft, tree_widths=(2,), prefill_step_size=16))[-1]
     assert 0 < last.prompt_tps < 1e7  # 200 tokens in 26 calls of the two models: not in 20 us
+
+
+def test_context_of_a_reused_cache():
+    """Tokens that a given cache holds count for the penalties and reach the grammar, once the caller names them."""
+    from myinfer_b200.generate import tree_speculative_generate_step
+    main, draft = _model(MAIN, 43), _model(DRAFT, 44)
+    V, before, prompt = MAIN["vocab_size"], [7, 8, 9, 7, 50], [11, 12]
+    seen = []
+
+    def grammar(tokens, nodes, parents):
+        seen.append(list(tokens))
+        return torch.full((len(nodes), V // 32), -1, dtype=torch.int32, device="cuda")
+
+    def run(**kw):
+        caches = [_prefilled(m, before, None) for m in (main, draft)]
+        seen.clear()
+        return [t for t, _ in tree_speculative_generate_step(
+            prompt, main, draft, (2, 1), 6, penalties=(1.0, 1000.0, 0.0), logit_bias={7: 50.0, 1500: 40.0}, grammar=grammar,
+            prompt_cache=caches[0], draft_cache=caches[1], **kw)]
+    got = run(context_tokens=before)
+    # token 7 has been said: 1000 less; 1500 is said once
+    assert 7 not in got and got[0] == 1500 and 1500 not in got[1:]
+    assert seen[0] == before + prompt[:-1]
+    assert run()[0] == 7 and seen[0] == prompt[:-1]  # without them only the prompt counts
+    for bad in (before[:-1], before + [1], [7, 8, 9, 7, V], [7, 8, 9, 7, -1]):
+        with pytest.raises(ValueError, match="context_tokens"):
+            run(context_tokens=bad)
