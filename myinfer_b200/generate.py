@@ -422,7 +422,7 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
     logits = torch.empty(T, V, dtype=torch.bfloat16, device=dev)
     d_logits = torch.empty(max(len(lv) for lv in levels), V, dtype=torch.bfloat16, device=dev)
     lengths = torch.zeros(1, dtype=torch.int32, device=dev)
-    tables, sig = None, None
+    tables = None
     ntoks = 0
     if stats is not None:
         torch.cuda.current_stream(dev).synchronize()  # the prompt has run: its time ends here
@@ -450,8 +450,7 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
             logits[:, 0] = torch.where(picks < 0, 0.0, logits[:, 0])  # the sampler takes no row of -inf's alone
             picks = torch.where(picks < 0, picks, sampler(logits))    # a node the grammar leaves nothing stays -1
         path, n, nxt = tree_accept(parents, tokens, picks.reshape(1, T), counts=counts)
-        if sig != (mcache.signature(), dcache.signature()):
-            tables, sig = (CacheLayers(mcache), CacheLayers(dcache)), (mcache.signature(), dcache.signature())
+        tables = tables or (CacheLayers(mcache), CacheLayers(dcache))
         lengths.fill_(mcache.offset)
         for t in tables:
             commit_tree(t, lengths, path, n)

@@ -111,23 +111,38 @@ def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, picks: torch.Tensor
 
 
 class CacheLayers:
-    """Table of a cache's buffers for ``commit_tree``: a ``PromptCache``, or
-    (keys, values) per layer with the shapes ``tree_attention`` takes (buffers
-    contiguous).  Build it again when the cache reallocates."""
+    """Table of a cache's buffers for ``commit_tree``: a ``PromptCache`` (or a list
+    of its layers), whose buffers it follows when they are reallocated or quantized,
+    or (keys, values) per layer with the shapes ``tree_attention`` takes (buffers
+    contiguous; these very tensors, which the table keeps alive)."""
 
     def __init__(self, layers):
+        # the list and what it held: layers and the generations of their buffers
+        self._source = layers if isinstance(layers, list) and all(hasattr(c, "generation") for c in layers) else None
+        self._fill(layers)
+
+    def current(self) -> tuple:
+        """``call``, after filling the table again if the cache's buffers have moved."""
+        src = self._source
+        if src is not None and (self._layers != src or self._generations != [c.generation for c in src]):
+            self._fill(src)
+        return self.call
+
+    def _fill(self, layers):
         pairs: List[tuple] = [(c.keys, c.values) if hasattr(c, "keys") else tuple(c) for c in layers]
         if not pairs:
             raise ValueError("no cache layers")
-        self._keep = pairs  # the table holds addresses only
         arr = (M5LayerKv * len(pairs))()
         shape = None
         for a, (k, v) in zip(arr, pairs):
+            if k is None or v is None:
+                raise ValueError("a cache layer without buffers")
             packed = not isinstance(k, torch.Tensor)
             ks, vs = (tuple(k), tuple(v)) if packed else ((k,), (v,))
             data = ks[0]
             for t in ks + vs:
-                if not t.is_cuda or not t.is_contiguous() or t.dim() != 4 or t.shape[:3] != data.shape[:3]:
+                if not t.is_cuda or t.device != data.device or not t.is_contiguous() or t.dim() != 4 or \
+                        t.shape[:3] != data.shape[:3]:
                     raise ValueError("cache buffers must be contiguous CUDA tensors [batch, kv heads, rows, ...]")
             if packed:
                 if len(ks) != 3 or len(vs) != 3 or ks[0].dtype != torch.int32 or vs[0].dtype != torch.int32 or \
@@ -153,14 +168,17 @@ class CacheLayers:
         self.batch, self.kv_heads, self.head_dim = shape
         if self.head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {self.head_dim}")
-        self.structs = arr
+        self.structs, self._keep = arr, pairs  # the table holds addresses only
         self.call = (ctypes.addressof(arr), len(arr), self.batch, self.kv_heads, self.head_dim, self.device.index)
+        if self._source is not None:
+            self._layers, self._generations = list(layers), [c.generation for c in layers]
 
 
 def commit_tree(layers, lengths: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor) -> None:
     """Keep an accepted path (``tree_accept``): in every layer, row ``lengths[b]
     + path[b, i]`` of K and V becomes row ``lengths[b] + i``, i < accepted[b], in
-    place.  ``layers``: a ``CacheLayers`` (a loop keeps one), or what it takes.
+    place.  ``layers``: a ``CacheLayers`` (a loop keeps one), or what it takes; a
+    captured graph keeps the buffers of its capture.
     ``lengths`` is left to the caller to advance."""
     t = layers if isinstance(layers, CacheLayers) else CacheLayers(layers)
-    (_calls or _load()).commit(*t.call, lengths, path, accepted)
+    (_calls or _load()).commit(*t.current(), lengths, path, accepted)

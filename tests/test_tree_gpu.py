@@ -717,3 +717,37 @@ def test_attention_broken_committed_key(bits):
         assert torch.isnan(out[..., :64]).all()
         out = _attend(q, put(k, -math.inf, at), v, [n], words, 0.05, T, bits)
         _check(out, q, without(k, at), without(v, at), [n - 1], words, 0.05, T, bits)
+
+
+@pytest.mark.parametrize("change", ["reserve", "quantize", "list"])
+def test_commit_follows_a_reallocated_cache(change):
+    """A table of a cache whose buffers have moved since it was made: the rows move in the buffers of now."""
+    from myinfer_b200.cache import KVCache, PromptCache
+    from myinfer_b200.tree import CacheLayers, commit_tree
+    g = torch.Generator(device="cuda").manual_seed(1)
+    layers = [KVCache(2, 128, "cuda", 256) for _ in range(3)]
+    cache = layers if change == "list" else PromptCache(layers, "cuda")
+    for c in cache:
+        c.update_and_fetch(*(torch.randn(1, 2, 40, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)))
+    table = CacheLayers(cache)
+    args = [torch.tensor(x, dtype=torch.int32).cuda() for x in ([30], [[0, 2, 5, -1, -1, -1]], [3])]
+    for i, c in enumerate(cache):
+        if change == "quantize":
+            cache[i] = c.to_quantized(64, 8)
+        else:
+            c.reserve(1000)
+    old = [[x.clone() for x in c._tensors()] for c in cache]
+    commit_tree(table, *args)
+    for c, before in zip(cache, old):
+        for x, o in zip(c._tensors(), before):
+            o[:, :, 31], o[:, :, 32] = o[:, :, 32].clone(), o[:, :, 35].clone()
+            assert torch.equal(x, o)
+
+
+def test_commit_refuses_a_cache_without_buffers():
+    from myinfer_b200.cache import KVCache, PromptCache
+    from myinfer_b200.tree import CacheLayers
+    with pytest.raises(ValueError, match="without buffers"):
+        CacheLayers(PromptCache([KVCache(2, 128, "cuda")], "cuda"))
+    with pytest.raises(ValueError, match="no cache layers"):
+        CacheLayers(PromptCache([], "cuda"))
