@@ -5,12 +5,13 @@ compiled for ``sm_100a`` only (``-gencode arch=compute_100a,code=sm_100a``),
 without fast-math (the KV quantizer must round exactly like the CPU rule),
 and linked into ``myinfer_b200/libm5cuda.so`` next to this file.
 ``csrc/tree_binding.cpp`` (the Python entries of the tree operators, against torch's
-headers) becomes ``myinfer_b200/_tree_binding.so``.
+headers) becomes ``myinfer_b200/_tree_binding.so``, after the library, which needs neither.
 """
 
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -87,8 +88,16 @@ def build_binding() -> Path:
 
 
 def build(verbose: bool = False) -> Path:
+    build_library(verbose)
+    if importlib.util.find_spec("torch") is not None:
+        build_binding()
+    else:
+        print(f"no torch: {BINDING.name} (Python entries of the tree operators) is not built", file=sys.stderr)
+    return LIB
+
+
+def build_library(verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
-    build_binding()
     srcs = sorted(CSRC.glob("*.cu"))
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
