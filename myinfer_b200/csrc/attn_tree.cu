@@ -29,15 +29,19 @@
 //                stream and take half of a tile's keys each; they only exchange maxima when
 //                one of them moves (a barrier with an OR tells).  S is double buffered
 //                within a stream and P overwrites the S it came from.
-// Rounding: K, V and P are fp16 (2^-12 of the value or less; bf16 would cost as
-// much as the output's own rounding).  The exponents make that safe for
-// any range: an element's absolute error is at most 2^-23 of its tile's largest
-// value.  Q is scaled per row in the same way, which is exact.  Scores, maxima,
+// Rounding: K, V and P are fp16 (2^-11 of the value; bf16 would cost as
+// much as the output's own rounding).  The exponents make that safe for any range:
+// below fp16's normal numbers an element is off by half a unit, 2^-25, where the
+// largest of K's tile, and of V's tiles in this run so far (O can follow an exponent
+// up, not down: it might overflow), is held at 2^-3 or more for codes and 2^7 for bf16.
+// That is 2^-22 of the largest, twice for codes with the rounding of their bias, and 2^-32 for bf16:
+// a value 2^12 below another one of its run is right to 2^-9 of itself, a bf16's rounding.
+// Q is scaled per row in the same way, which is exact.  Scores, maxima,
 // sums and O are fp32.  Infinities and NaN stay what they are and have no part in the
 // exponents; the V of a tree key that holds one is zeroed and the queries that see the key
 // are made NaN at the run's end, so that the others do not meet 0 times it (64 nodes over
-// 32768 keys 98.9 us with it, 97.5 without; bf16 127.3, 123.2).  A row's maximum is only moved when a new score exceeds
-// it by 2^8 (p <= 256 in fp16): O is rescaled rarely.
+// 32768 keys 98.9 us with it, 97.5 without; bf16 127.3, 123.2).  A row's maximum is only
+// moved when a new score exceeds it by 2^8 (p <= 256 in fp16): O is rescaled rarely.
 // TMEM columns: S / P [stream][2] 64 each, O [stream] 128 each (all 512).
 //
 // Time on the device (launches in a graph, inputs of 3 sets in turn): 2 rows a kv head over
@@ -394,7 +398,7 @@ struct Row {
 
 // One tile of a softmax thread: N of the tile's 64 keys, from `off` on, into the P
 // columns of those keys.  pair: barrier of the two warps that share the
-// rows (0: this warp has them alone), mine / other: where they exchange maxima.
+// rows, mine / other: where they exchange maxima.
 // Returns the factor by which O has to change.
 __device__ __forceinline__ float softmax_tile(Row& r, uint32_t s_addr, int off, float c, bool edge,
                                               unsigned long long vis, int pair, float* mine, const float* other) {

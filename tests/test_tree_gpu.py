@@ -751,3 +751,35 @@ def test_commit_refuses_a_cache_without_buffers():
         CacheLayers(PromptCache([KVCache(2, 128, "cuda")], "cuda"))
     with pytest.raises(ValueError, match="no cache layers"):
         CacheLayers(PromptCache([], "cuda"))
+
+
+@pytest.mark.parametrize("bits", [0, 4, 8])
+@pytest.mark.parametrize("n", [500, 9000])
+def test_attention_shrinking_values(bits, n):
+    """Values of 2^12 first, at keys that weigh nothing, and of 1 behind them.  In fp16 a value is off by u of itself
+    or, far below the largest of its run so far, by half a subnormal unit, 2^-25.  The largest is held at 2^-3 or more
+    for codes, whose bias is rounded too (2 x 2^-22 of the largest), and at 2^7 or more for bf16 (2^-32)."""
+    rng = np.random.default_rng(13)
+    L = T = 3
+    D, big, first = 64, 2.0 ** 12, 20
+    q = np.abs(rng.standard_normal((1, 2, L, D))) + 0.5
+    kx = rng.standard_normal((1, 1, n + T, D)).astype(np.float32)
+    kx[:, :, :first] = -6.0                      # scores below the others' by hundreds
+    vx = rng.standard_normal((1, 1, n + T, D)).astype(np.float32)
+    vx[:, :, :first] *= big
+    q = _bf(q).cuda()
+    k, v = ((_pack(kx, bits), _pack(vx, bits)) if bits else (_bf(kx), _bf(vx)))
+    words = ref.ancestors(_trees(rng, 1, T))[0]
+    out = _f64(_attend(q, k, v, [n], words, 0.25, T, bits))
+    kd, vd = _dense(k, bits), _dense(v, bits)
+    want, mag = ref.attention(_f64(q)[0], kd[0], vd[0], n, words[0], T, 0.25)
+    if bits:
+        s, b = _f64(v[1]), _f64(v[2])
+        unit = 2.0 ** -21 * max(np.abs(b).max(), np.abs(s * (2 ** bits - 1) + b).max())
+    else:
+        unit = 2.0 ** -32 * np.abs(vd).max()
+    for h in range(2):
+        d = 8 / math.sqrt(3) * U * 0.25 * np.sqrt((_f64(q)[0, h] ** 2) @ (kd[0, 0] ** 2).T).max(1)
+        tol = 2.0 ** -8 * np.abs(want[h]) + unit + (np.expm1(2 * d) + 4 * U)[:, None] * mag[h]
+        err = np.abs(out[0, h] - want[h])
+        assert (err <= tol).all(), float((err - tol).max())
