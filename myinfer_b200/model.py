@@ -288,6 +288,13 @@ class Model:
                             (ancestors, torch.int64, "ancestors")):
             if t.dtype is not dt or t.numel() != L or not t.is_cuda or not t.is_contiguous():
                 raise ValueError(f"forward_tree: {what} must be {L} contiguous {dt} values on the device")
+        if cache.batch != 1:
+            raise ValueError(f"forward_tree takes a cache of one sequence, not of {cache.batch}")
+        if logits_mode != _lib.M5_LOGITS_NONE:
+            n = self.args.vocab_size * (L if logits_mode == _lib.M5_LOGITS_ALL else 1)
+            if logits is None or logits.dtype is not torch.bfloat16 or not logits.is_cuda or \
+                    not logits.is_contiguous() or logits.numel() < n:
+                raise ValueError(f"forward_tree: logits must be {n} or more contiguous bf16 values on the device")
         if L > self.max_tokens:
             self.reserve(L)
         need = cache.offset + row0 + L

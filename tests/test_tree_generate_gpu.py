@@ -268,3 +268,27 @@ def test_context_of_a_reused_cache():
     for bad in (before[:-1], before + [1], [7, 8, 9, 7, V], [7, 8, 9, 7, -1]):
         with pytest.raises(ValueError, match="context_tokens"):
             run(context_tokens=bad)
+
+
+def test_forward_tree_refusals():
+    """A logits buffer that the call would write past, or of another type, and a cache of several sequences."""
+    from myinfer_b200 import _lib
+    from myinfer_b200.cache import KVCache, PromptCache, make_prompt_cache
+    from myinfer_b200.tree import tree_plan
+    main = _model(MAIN, 37)
+    V = MAIN["vocab_size"]
+    anc, depth = tree_plan(torch.tensor([[-1, 0, 0]], dtype=torch.int32).cuda())
+    tok = torch.zeros(3, dtype=torch.int32, device="cuda")
+    cache = make_prompt_cache(main, 64)
+    new = lambda *s, **kw: torch.empty(*s, **{**dict(dtype=torch.bfloat16, device="cuda"), **kw})  # noqa: E731
+    for mode, lg in ((_lib.M5_LOGITS_ALL, new(2, V)), (_lib.M5_LOGITS_ALL, new(3, V, dtype=torch.float32)),
+                     (_lib.M5_LOGITS_ALL, new(3, V, device="cpu")), (_lib.M5_LOGITS_ALL, new(3, 2 * V)[:, :V]),
+                     (_lib.M5_LOGITS_ALL, None), (_lib.M5_LOGITS_LAST, new(V - 1))):
+        with pytest.raises(ValueError, match="logits"):
+            main.forward_tree(tok, cache, depth[0], anc[0], 0, mode, lg)
+    batch = PromptCache([KVCache(main.n_kv_heads_local, 128, "cuda", 64, batch=2) for _ in range(3)], "cuda")
+    with pytest.raises(ValueError, match="one sequence"):
+        main.forward_tree(tok, batch, depth[0], anc[0])
+    main.forward_tree(tok, cache, depth[0], anc[0], 0, _lib.M5_LOGITS_LAST, new(V))
+    main.forward_tree(tok, cache, depth[0], anc[0], 0, _lib.M5_LOGITS_ALL, new(5, V))
+    _lib.device_check()
