@@ -355,7 +355,8 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
                                    draft_cache: Optional[PromptCache] = None, prefill_step_size: int = 2048,
                                    kv_bits: Optional[int] = None, kv_group_size: int = 64,
                                    quantized_kv_start: int = 0, stats: Optional[dict] = None,
-                                   context_tokens: Optional[List[int]] = None) -> Iterator[tuple]:
+                                   context_tokens: Optional[List[int]] = None,
+                                   logits_processors: Optional[list] = None) -> Iterator[tuple]:
     """Speculative decoding over a tree of drafts: each round the draft model
     proposes, for every node of a level, its ``tree_widths[d]`` likeliest tokens,
     the main model scores all nodes in one call, and the longest path whose
@@ -366,7 +367,8 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
     decode (with the same processors).
 
     ``sampler``: a ``DeviceSampler`` draws the choices from the processed logits
-    (its own penalty window is not used).  ``penalties`` = (repetition, presence,
+    (its own penalty window is not used, and ``logits_processors``, penalties over a
+    window, must be empty).  ``penalties`` = (repetition, presence,
     frequency) over the context: the prompt, what is generated, and ``context_tokens``,
     the tokens that a given ``prompt_cache`` already holds (all of them, in order; left
     out, they do not count).  ``logit_bias`` maps token ids to added
@@ -382,7 +384,7 @@ def tree_speculative_generate_step(prompt: List[int], model, draft_model, tree_w
         raise ValueError(f"token id out of range [0, {V})")
     if sampler is not None and not isinstance(sampler, DeviceSampler):
         raise ValueError("tree speculation samples with a DeviceSampler (make_sampler) or greedily")
-    if sampler is not None and sampler.window:
+    if logits_processors or (sampler is not None and sampler.window):
         raise ValueError("give penalties to tree speculation itself: a node's window is its own path")
     levels = tree_shape(tree_widths)
     T = sum(len(lv) for lv in levels)

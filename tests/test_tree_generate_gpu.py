@@ -292,3 +292,23 @@ def test_forward_tree_refusals():
     main.forward_tree(tok, cache, depth[0], anc[0], 0, _lib.M5_LOGITS_LAST, new(V))
     main.forward_tree(tok, cache, depth[0], anc[0], 0, _lib.M5_LOGITS_ALL, new(5, V))
     _lib.device_check()
+
+
+def test_processors_of_the_other_loops():
+    """What a caller of every loop passes, an empty list of logits processors, is taken; penalties over a window are
+    refused with the reason."""
+    from myinfer_b200.generate import stream_generate
+    from myinfer_b200.sample import make_logits_processors
+
+    class Tok:
+        eos_token_ids = []
+
+        def decode(self, ids):
+            return " ".join(str(i) for i in ids)
+    main, draft = _model(MAIN, 31), _model(DRAFT, 32)
+    kw = dict(max_tokens=4, draft_model=draft, tree_widths=(2,), prefill_step_size=16)
+    want = [r.token for r in stream_generate(main, Tok(), [3, 1, 4], **kw)]
+    for none in (None, make_logits_processors()):
+        assert [r.token for r in stream_generate(main, Tok(), [3, 1, 4], logits_processors=none, **kw)] == want
+    with pytest.raises(ValueError, match="penalties"):
+        next(stream_generate(main, Tok(), [3, 1, 4], logits_processors=make_logits_processors(1.2), **kw))
