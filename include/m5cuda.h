@@ -291,7 +291,10 @@ M5_API int m5_tree_attention_workspace(int B, int Hq, int Hkv, int L, int D, siz
  * do not exist.  Rows no query sees are not used, whatever they hold; a row with
  * NaN or an infinity makes NaN or infinities of the queries that see it (the whole
  * row NaN where it is a tree key's value), and is nothing to the others.
- * Scores, maxima and sums are fp32; nothing is rounded to bf16 before the output.
+ * Keys, values and weights are used in fp16 under an exponent of their tile or run (2^-11 of the
+ * value; far below the largest 2^-21 of that for codes), queries under one of their row (exact);
+ * scores, maxima and sums are fp32, and nothing is rounded to bf16 before the output.
+ * Of scales and biases the 16-byte blocks that hold a head's first and last are read whole.
  * workspace: 16-byte aligned, not shared by calls that may overlap. */
 M5_API int m5_tree_attention(const void* q, const int64_t* q_strides, int B, int Hq, int L, int D, m5_kv_view keys,
                              m5_kv_view values, int Hkv, int64_t capacity, const int32_t* lengths, int tree_len,

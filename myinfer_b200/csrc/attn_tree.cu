@@ -39,22 +39,22 @@
 // Q is scaled per row in the same way, which is exact.  Scores, maxima,
 // sums and O are fp32.  Infinities and NaN stay what they are and have no part in the
 // exponents; the V of a tree key that holds one is zeroed and the queries that see the key
-// are made NaN at the run's end, so that the others do not meet 0 times it (64 nodes over
-// 32768 keys 98.9 us with it, 97.5 without; bf16 127.3, 123.2).  A row's maximum is only
+// are made NaN at the run's end, so that the others do not meet 0 times it (512 rows over
+// 32768 keys 98.9 us with it, 97.5 without; bf16 127.4, 123.2).  A row's maximum is only
 // moved when a new score exceeds it by 2^8 (p <= 256 in fp16): O is rescaled rarely.
 // TMEM columns: S / P [stream][2] 64 each, O [stream] 128 each (all 512).
 //
 // Time on the device (launches in a graph, inputs of 3 sets in turn): 2 rows a kv head over
-// 512 keys 12.8 us (two launches, one tile per CTA and a join: latency); 128 rows x 8 kv heads over
+// 512 keys 13.0 us (two launches, one tile per CTA and a join: latency); 128 rows x 8 kv heads over
 // 131072 keys, 4 bits: 105 us = 654 TFLOP/s, 1.44 TB/s; 512 rows x 8 kv heads over 32768 keys, 8
-// bits: 97 us = 710 TFLOP/s.  Long calls are bound by the chain of hand-overs of a tile (a
+// bits: 98.9 us = 696 TFLOP/s.  Long calls are bound by the chain of hand-overs of a tile (a
 // poll of a complete barrier takes 80-190 cycles, commit to wait 230) together with the issue
-// slots: at 512 rows 61 % of the slots, tensor cores 57 % of the cycles at the 1.64 GHz the
-// power limit leaves, DRAM 10 %; a copy without any arithmetic in conversion and softmax still
-// took 64-70 us.  What did not pay: 8 softmax warps (110 us at 512 rows), one lane polling for its warp
-// (166), S and PV from two warps (113), one thread as MMA warp with its waits polled ahead (104),
-// 128 keys per hand-over (104: a stream's next S then waits for its PV), few rows repeated over
-// the idle lanes of a tile (103; one node over 512 keys 13.7).
+// slots: at 512 rows 61 % of the slots, tensor cores 56 % of the cycles, DRAM 10 %; a copy without any
+// arithmetic in conversion and softmax still took 64-70 us.  What did not pay, at 512 rows (96 us then):
+// 8 softmax warps (110), one lane polling for its warp (166), S and PV from two warps (113), one
+// thread as MMA warp with its waits polled ahead (104), 128 keys per hand-over (104: a stream's
+// next S then waits for its PV).  Few rows: repeated over the idle lanes of a tile, 8 rows over
+// 32768 keys 38.7 (36.2 then; 37.5 now).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -250,7 +250,7 @@ __device__ __forceinline__ int part_with(int total, int ctas, int t) {
   return c;
 }
 // parts of the line: down to one tile each (a CTA's second tile costs more than a part to join: one
-// node over 512 keys 17.0 us with at least two tiles, 13.9 with one)
+// node over 512 keys 16.3 us with at least two tiles, 13.0 with one)
 __device__ __forceinline__ int parts(int total, int ctas) { return ::min(ctas, total); }
 // by one warp: this CTA's part of the line
 __device__ __forceinline__ Line part_of_line(const TreeAttnArgs& a, int pairs, int lane, int c, int ctas) {
@@ -1206,9 +1206,9 @@ struct Plan {
 static Plan plan(int B, int Hq, int Hkv, int L) {
   const long long rows = (long long)L * (Hq / Hkv);
   // Two blocks of rows per converted tile (one: two parts convert each tile) from 129 rows on, over
-  // 32768 keys: 256 rows 58.8 us (one: 62.9), 512 rows 95.0 (112.7), bf16 122.5 (176.7); 128 rows
-  // 49.1 (one: 42.7), the second stream idle.  Over 600 keys one would do: 256 rows 19.0 (16.1), 512
-  // 25.8 (26.0); the lengths are not known here.
+  // 32768 keys: 256 rows 61.8 us (one: 65.9), 512 rows 98.9 (118.4), bf16 127.4 (184.8); 128 rows
+  // 51.3 (one: 43.9), the second stream idle.  Over 600 keys one would do: 256 rows 19.4 (16.0), 512
+  // 26.1 (26.2); of the lengths only the capacity is known here, which a loop reserves ahead of them.
   const int blocks = rows > ROWS ? 2 : 1, nrb = ceil_div(rows, ROWS * blocks), ctas = sm_count();
   return {nrb, blocks, ctas, (size_t(ctas) + size_t(B) * Hkv * nrb) * blocks};
 }

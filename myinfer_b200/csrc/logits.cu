@@ -21,10 +21,10 @@
 // is the one that writes, so no order of threads matters.  The row's choice is a
 // maximum over (value, lowest index) words, joined over the cluster in shared memory.
 //
-// On the device: one bf16 row of 151936 with penalties 5.8 us (latency: loads, cluster join);
-// a tree of 64 such rows with 300 biases and masks 28.2 us (40.7 MB from and to memory, 1.44 TB/s;
+// On the device: one bf16 row of 151936 with penalties 5.9 us (latency: loads, cluster join);
+// a tree of 64 such rows with 300 biases and masks 28.6 us (40.7 MB from and to memory, 1.42 TB/s;
 // the counts, read again for every row from L2, take 7 us of it, the biases 6.5, the masks 2.5,
-// a plain copy 10); 40 fp32 rows of 32001, unaligned, 13.3 us.
+// a plain copy 10); 40 fp32 rows of 32001, unaligned, 12.9 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -431,7 +431,7 @@ extern "C" int m5_process_logits(const void* logits, int64_t ld, void* out, int6
   a.T = T;
   a.V = (int)vocab;
   // CTAs of a row: all rows at once on the SMs (two CTAs each), a power of two up to the cluster's
-  // 16 (7 CTAs for 40 rows of 32001 left SMs without a whole cluster: 17.8 us, 4 CTAs 12.7), parts
+  // 16 (7 CTAs for 40 rows of 32001 left SMs without a whole cluster: 17.8 us, 4 CTAs 12.9), parts
   // of 4096 to 65536 entries.  One row of 151936: 8 CTAs 8.0 us, 16 CTAs 5.9.
   const int64_t fit = 2 * sm_count() / (int64_t(B) * T);
   int ctas = 1;

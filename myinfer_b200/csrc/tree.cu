@@ -18,8 +18,8 @@
 //               layers: 8 KB of it cost the host 0.5 us more than 2).
 // None of them moves enough bytes to matter (a commit of 20 rows over 64 layers
 // is 5 MB): they are bound by their launch and by one to three dependent trips to
-// memory.  Accepting, one tree of 8 or 64 trees of 64 nodes: 2.0 us on the device.  A
-// commit of 28 layers, 8 heads, 8 bits: 3.2 us; of 64 layers for 4 requests, 4 bits: 5.9 us
+// memory.  Accepting, one tree of 8 or 64 trees of 64 nodes: 1.9-2.0 us on the device.  A
+// commit of 28 layers, 8 heads, 8 bits: 3.0 us; of 64 layers for 4 requests, 4 bits: 5.8 us
 // (11 MB, 1.9 TB/s).
 #include <algorithm>
 

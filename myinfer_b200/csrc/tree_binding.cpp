@@ -3,8 +3,8 @@
 //
 // A small call's kernels take 2 us (accepting a path) to 13 us (attention over a
 // short cache), so what the host does before them is the call's time: accepting
-// took 13.0 us a call with ctypes and takes 6.5, a commit of 28 layers 11.0 and 7.5,
-// one row of logits 12.7 and 8.2, attention over 512 keys 22.2 and 13.1 (its kernels).
+// took 13.0 us a call with ctypes and takes 6.4-6.9, a commit of 28 layers 11.0 and 7.2-7.8
+// (of a table already made), one row of logits 12.7 and 8.2, attention over 512 keys 22.2 and 13.3 (its kernels).
 // The kernels and the C ABI are libm5cuda.so's, whose addresses `bind` receives.  Errors
 // are ValueError for what a tensor must be, and the library's status through the
 // `check` that `bind` receives too.
